@@ -418,6 +418,28 @@ int mole_store_to_host(mole_ctx* ctx, void* host_dst, const void* dev_src, int64
 int mole_adam_update(void* p, void* m, void* v, const void* g, const void* g_extra, int64_t n,
                      int32_t dtype, float beta1, float beta2, int32_t t, float lr, float lam,
                      float eps, int32_t adamw, void* stream);
+/* One step over a list of tensors in one launch per 500 tensors.  p and g have element type `dtype`;
+ * the moments have `state_bits` bits: 32 = fp32 arrays, 8 = e4m3 codes with one fp32 scale per 256
+ * consecutive elements (m_scale, v_scale: [ceil(n / 256)]; m = code * m_scale, v = (code * v_scale)^2;
+ * all zero is a fresh state).  8-bit states are rounded up or down at random, by bits that depend on
+ * (seed, t, index in the list, element) alone.  A block whose largest moment is below 2^-100 is held
+ * as zeros; a moment that is NaN stays so and one that is infinite is held as its block's largest
+ * code, neither touching its neighbours.  t, lr and the rest as in mole_adam_update.  The list is a
+ * host array, read before the call returns.  Pointers need the alignment of their elements only
+ * (16 bytes, 8 for 8-bit moments, for the wide accesses).  t and lr are taken by value, so a stream
+ * under capture is refused (MOLE_ERR_STATE).  A tensor may appear once per call. */
+typedef struct {
+  void* p;
+  const void* g;
+  void* m;
+  void* v;
+  float* m_scale;         /* 8-bit moments only */
+  float* v_scale;
+  int64_t n;              /* elements, < 2^34; 0: skipped */
+} mole_adam_tensor;
+int mole_adam_multi(const mole_adam_tensor* tensors, int32_t n_tensors, int32_t dtype,
+                    int32_t state_bits, double beta1, double beta2, int32_t t, double lr, double lam,
+                    double eps, int32_t adamw, uint32_t seed, void* stream);
 /* P free pool slots, n layers, layer i can hide F[i] expert fetches and owns E[i] offloaded
  * experts.  local[i] = experts layer i prefetches for itself; triples[3j..3j+2] = (lender layer,
  * borrower layer, count): while the lender runs it also fetches `count` experts of the borrower.

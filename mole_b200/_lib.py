@@ -33,6 +33,10 @@ class FfnDesc(C.Structure):
         "n_slots", "n_grad_slots", "accumulate", "compact", "backend")]
 
 
+class AdamTensor(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("p", "g", "m", "v", "m_scale", "v_scale")] + [("n", C.c_int64)]
+
+
 _p, _i32, _i64 = C.c_void_p, C.c_int32, C.c_int64
 _pi32, _pi64 = C.POINTER(C.c_int32), C.POINTER(C.c_int64)
 
@@ -112,6 +116,8 @@ SIGNATURES = {
     "mole_store_to_host": (C.c_int, [_p, _p, _p, _i64, _p]),
     "mole_adam_update": (C.c_int, [_p, _p, _p, _p, _p, _i64, _i32, C.c_float, C.c_float, _i32,
                                    C.c_float, C.c_float, C.c_float, _i32, _p]),
+    "mole_adam_multi": (C.c_int, [C.POINTER(AdamTensor), _i32, _i32, _i32, C.c_double, C.c_double, _i32,
+                                  C.c_double, C.c_double, C.c_double, _i32, C.c_uint32, _p]),
     "mole_fast_assign_prefetch": (C.c_int, [_i32, _pi32, _pi32, _i32, _pi32, _pi32, _i32, _pi32]),
 }
 

@@ -6,6 +6,7 @@ None of them has a PyTorch fallback.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import math
 from dataclasses import dataclass
@@ -14,7 +15,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import FfnDesc, check, lib
+from ._lib import AdamTensor, FfnDesc, check, lib
 
 _DTYPES = {torch.float32: _lib.MOLE_F32, torch.bfloat16: _lib.MOLE_BF16}
 _ACTS = {"gelu": _lib.ACT_GELU, "relu": _lib.ACT_RELU}
@@ -42,6 +43,19 @@ def _stream() -> int:
     # the raw handle of the current stream of the current device; torch.cuda.current_stream()
     # builds a Stream object through several Python layers (17 us a call, a dozen calls a step)
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+
+
+def _on_device_of(first: torch.Tensor, *others: Optional[torch.Tensor]):
+    """Context in which the current device is the one all these tensors are on."""
+    dev = first.device
+    if dev.type != "cuda":
+        raise RuntimeError("mole_b200 kernels take CUDA tensors only (there is no CPU path)")
+    for t in others:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors are on different devices: {dev} and {t.device}")
+    if dev.index == torch._C._cuda_getDevice():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
 
 
 def capacity(T: int, E: int, k: int, capacity_factor: float) -> int:
@@ -296,6 +310,75 @@ def ffn_bwd_peer(desc: FfnDesc, counts, dout, x, x1, h, w1, w2, dx1, peer, gw1, 
                                 _ptr(x1), _ptr(h), _ptr(w1), _ptr(w2), _ptr(dx1), peer.table["dx"],
                                 peer.rank, _ptr(gw1), _ptr(gb1), _ptr(gw2), _ptr(gb2), _ptr(ws),
                                 ws.numel(), _stream()))
+
+
+# ---- one Adam step over many tensors ---------------------------------------------------------
+ADAM_BLOCK = 256      # elements of an 8-bit moment that share one scale
+
+
+def adam_scales(numel: int) -> int:
+    """Number of scales of an 8-bit moment of ``numel`` elements."""
+    return -(-numel // ADAM_BLOCK)
+
+
+def adam_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
+               exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor],
+               m_scales: Optional[Sequence[torch.Tensor]] = None,
+               v_scales: Optional[Sequence[torch.Tensor]] = None, *, t: int, lr: float,
+               betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0,
+               adamw: bool = True, seed: int = 0) -> None:
+    """One Adam / AdamW step over a list of tensors, in place, in one launch per 500 tensors.
+
+    ``t`` is the step count after this step.  Parameters and gradients are all float32 or all
+    bfloat16; the moments are all float32, or all ``torch.float8_e4m3fn`` with a float32 scale per
+    256 consecutive elements in ``m_scales`` / ``v_scales`` (``m = code * scale``,
+    ``v = (code * scale) ** 2``; zeros are a fresh state).  8-bit moments are rounded at random by
+    bits that ``seed``, ``t``, the place in the list and the element determine: the same call gives
+    the same bits."""
+    n = len(params)
+    lists = [params, grads, exp_avgs, exp_avg_sqs]
+    if n == 0:
+        return
+    bits = 8 if exp_avgs[0].dtype == torch.float8_e4m3fn else 32
+    if bits == 8:
+        if m_scales is None or v_scales is None:
+            raise ValueError("8-bit moments need m_scales and v_scales")
+        lists += [m_scales, v_scales]
+    elif m_scales is not None or v_scales is not None:
+        raise ValueError("32-bit moments have no scales")
+    if any(len(x) != n for x in lists):
+        raise ValueError("one gradient, two moments (and their scales) per parameter")
+    dt = _dt(params[0])
+    dtype, device = params[0].dtype, params[0].device
+    mdtype = torch.float8_e4m3fn if bits == 8 else torch.float32
+    table = (AdamTensor * n)()
+    seen = set()
+    for i, ts in enumerate(zip(*lists)):
+        p, g, m, v = ts[:4]
+        size = p.numel()
+        if p.dtype != dtype or g.dtype != dtype:
+            raise TypeError(f"tensor {i}: parameter and gradient must both be {dtype}")
+        if m.dtype != mdtype or v.dtype != mdtype:
+            raise TypeError(f"tensor {i}: both moments must be {mdtype}")
+        if g.numel() != size or m.numel() != size or v.numel() != size:
+            raise ValueError(f"tensor {i}: parameter, gradient and moments differ in size")
+        for x in ts:
+            if x.device != device:
+                raise ValueError(f"tensor {i}: tensors are on different devices: {device} and {x.device}")
+        e = table[i]
+        e.p, e.g, e.m, e.v, e.n = _ptr(p), _ptr(g), _ptr(m), _ptr(v), size
+        if bits == 8:
+            for x in ts[4:]:
+                if x.dtype != torch.float32 or x.numel() != adam_scales(size):
+                    raise ValueError(f"tensor {i}: scales must be float32 [{adam_scales(size)}]")
+            e.m_scale, e.v_scale = _ptr(ts[4]), _ptr(ts[5])
+        if size and (e.p in seen):
+            raise ValueError(f"tensor {i}: the same parameter twice in one call")
+        seen.add(e.p)
+    with _on_device_of(params[0]):
+        check(lib.mole_adam_multi(table, n, dt, bits, betas[0], betas[1], int(t), float(lr),
+                                  float(weight_decay), float(eps), int(bool(adamw)),
+                                  int(seed) & 0xffffffff, _stream()))
 
 
 def device_fault_poll() -> None:

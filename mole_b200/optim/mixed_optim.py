@@ -1,7 +1,9 @@
 """``MOLEMixedAdam``: one Adam over three parameter populations (interface of
 MOLE/optim/mixed_optim.py:155-343).
 
-  GPU-resident experts and the gate   ``torch.optim.Adam`` / ``AdamW`` on the device
+  GPU-resident experts and the gate   ``torch.optim.Adam`` / ``AdamW`` on the device, or -- with
+                                      ``state_bits`` -- ``DeviceAdam``: all tensors in one launch,
+                                      moments in 32 or 8 bits
   offloaded experts                   ``CPUAdam`` on the pinned host arrays, or -- with
                                       ``adv_adam`` -- the fused GPU step that ``MOLECore``
                                       runs right behind each expert batch's backward; then
@@ -17,6 +19,8 @@ from __future__ import annotations
 from copy import deepcopy
 
 import torch
+
+from .device_adam import DeviceAdam, unpack_moment
 
 
 class CPUAdam(torch.optim.Optimizer):
@@ -108,7 +112,7 @@ class CPUAdam(torch.optim.Optimizer):
 
 class MOLEMixedAdam:
     def __init__(self, CPUParams, GPUParams, GateParams, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
-                 weight_decay=0, adamW=False):
+                 weight_decay=0, adamW=False, state_bits=None, seed=0):
         self.GateParams = GateParams
         self.CPUParams = CPUParams
         self.GPUParams = GPUParams
@@ -119,6 +123,11 @@ class MOLEMixedAdam:
         kw = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
         if self.hasCPU:
             self.cpu_optimizer = CPUAdam(CPUParams, bias_correction=True, adamw_mode=adamW, **kw)
+        if state_bits is not None:
+            def dev_cls(params, **kw):
+                # the gate is small and decides the routing: its moments stay in 32 bits
+                return DeviceAdam(params, adamw_mode=adamW, seed=seed,
+                                  state_bits=32 if params is GateParams else state_bits, **kw)
         if self.hasGPU:
             self.gpu_optimizer = dev_cls(params=GPUParams, **kw)
         if self.hasGate:
@@ -128,10 +137,15 @@ class MOLEMixedAdam:
     @torch.no_grad()
     def get_optim_state(self):
         """``[expert_state, gate_state]``: per parameter kind the moments of the GPU-resident
-        experts followed by those of the offloaded ones (dimension 0), all on the host."""
+        experts followed by those of the offloaded ones (dimension 0), all on the host (8-bit moments
+        as the fp32 values they stand for)."""
         def host(opt):
             st = deepcopy(opt.state_dict()["state"])
             for k in st:
+                for name in ("exp_avg", "exp_avg_sq"):
+                    scale = st[k].pop(name + "_scale", None)
+                    if scale is not None:
+                        st[k][name] = unpack_moment(st[k][name], scale, name == "exp_avg_sq")
                 st[k]["exp_avg"] = st[k]["exp_avg"].cpu()
                 st[k]["exp_avg_sq"] = st[k]["exp_avg_sq"].cpu()
             return st

@@ -112,7 +112,9 @@ class UniScheduler:
     # ---- optimizer (MOLE/utils/Uscheduler.py:94-153) ----------------------------------------------
     @staticmethod
     def build_optimizer(lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0, gate_only=False,
-                        adamW=False):
+                        adamW=False, state_bits=None, seed=0):
+        """``state_bits`` (32 or 8): GPU-resident tensors are stepped by ``DeviceAdam`` instead of
+        ``torch.optim``; ``seed`` starts the random rounding of its 8-bit moments."""
         sched = UniScheduler._instance
         sched.adamW = adamW
         cpu_params, gpu_params, gate_params = [], [], []
@@ -127,7 +129,7 @@ class UniScheduler:
             cpu_params += UnifiedCPUTensor.get_cpu_experts()
         if cpu_params or gpu_params or gate_params:
             UniScheduler._optimizer = mixed_optim.MOLEMixedAdam(
-                cpu_params, gpu_params, gate_params, lr, betas, eps, weight_decay, adamW)
+                cpu_params, gpu_params, gate_params, lr, betas, eps, weight_decay, adamW, state_bits, seed)
         else:
             UniScheduler._optimizer = None
             return None
