@@ -302,6 +302,36 @@ int mole_ffn_bwd_peer(const mole_ffn_desc* desc, const int32_t* counts,
                       int64_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------
+ * products over rows packed by expert, without capacity, padding or a step of the FFN around them.
+ * Expert e owns rows [offsets[e], offsets[e + 1]) of the packed matrices (offsets int32 [E + 1] on
+ * the device, as mole_gate_route_fwd writes them; E <= 256; an expert may have no rows).  Rows before
+ * offsets[0] and from offsets[E] on belong to nobody: products write zeros there.  The offsets are
+ * clamped on the device to a rising sequence in [0, R].  Any width and element-aligned pointers are
+ * taken; widths that are multiples of 8 (16 for 8-bit integers) with 16-byte aligned pointers run on
+ * the tensor cores for bf16 and 8-bit integers.  All sums are held in 32 bits and rounded once.
+ * The reference computes the same products inside bffn_fwd / bffn_bwd over capacity-padded rows
+ * (MOLE/cpp/core.cpp:350-353, 388-412).
+ * ---------------------------------------------------------------------------------- */
+/* out[r, n] = sum_k x[r, k] w_e(n, k) for r of expert e: w is [E, N, K] (w_kn = 0) or [E, K, N]
+ * (w_kn = 1).  The gradient of x is the same call on dout with the other w_kn. */
+int mole_grouped_mm(const void* x, const void* w, const int32_t* offsets, int64_t R, int32_t N,
+                    int32_t K, int32_t E, int32_t w_kn, int32_t dtype, void* out, void* stream);
+/* out[e, p, q] = sum over the rows r of e of a[r, p] b[r, q]: the weight gradient, zeros for an expert
+ * without rows */
+int mole_grouped_mm_wgrad(const void* a, const void* b, const int32_t* offsets, int64_t R, int32_t P,
+                          int32_t Q, int32_t E, int32_t dtype, void* out, void* stream);
+/* q[r, k] = the integer in [-127, 127] nearest to x[r, k] / scale[r] (ties to even, decided exactly),
+ * scale[r] = max_k |x[r, k]| / 127 rounded to fp32.  A row with a value that is not finite gets a
+ * scale that is not finite and zeros: its products come out NaN. */
+int mole_quantize_rows(const void* x, int64_t R, int32_t K, int32_t dtype, void* q, float* scale,
+                       void* stream);
+/* out[r, n] = (sum_k q[r, k] w[e, n, k]) q_scale[r] w_scale[e, n]: int8 operands (w [E, N, K], K < 2^17),
+ * the sum exact in 32 bits, out in out_dtype.  offsets may be null for E = 1 (every row belongs to it). */
+int mole_grouped_mm_i8(const void* q, const float* q_scale, const void* w, const float* w_scale,
+                       const int32_t* offsets, int64_t R, int32_t N, int32_t K, int32_t E,
+                       int32_t out_dtype, void* out, void* stream);
+
+/* ------------------------------------------------------------------------------------
  * streams.  Replaces the 16-stream manager (MOLE/cpp/stream.cpp:38-144) and its wait
  * helpers (stream.cpp:156-205).  Roles follow the reference: 1 = H2D transfer, 2 = compute,
  * 3 = communication, 4 = D2H transfer.

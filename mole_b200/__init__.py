@@ -6,7 +6,7 @@ loads that library and fails loudly when it has not been built (``python mole_b2
 """
 from . import _lib, ops                      # noqa: F401  (loads the shared library)
 from .moe.layer import MOLEModule            # noqa: F401
-from .moe.functions import BatchFusedFWD, pfetchbwd   # noqa: F401
+from .moe.functions import BatchFusedFWD, grouped_mm, pfetchbwd   # noqa: F401
 from .utils.Ugate import MOLETopk            # noqa: F401
 
-__all__ = ["MOLEModule", "MOLETopk", "BatchFusedFWD", "pfetchbwd", "ops"]
+__all__ = ["MOLEModule", "MOLETopk", "BatchFusedFWD", "pfetchbwd", "grouped_mm", "ops"]

@@ -1,0 +1,146 @@
+// C entries of the products over rows packed by expert, and the quantisation of rows to 8-bit
+// integers that the integer product takes.
+#include "ragged.cuh"
+
+namespace mole {
+
+// ---- rows to 8-bit integers ------------------------------------------------------------------
+// scale = max |x| / 127 rounded to fp32; q = the integer nearest to x / scale, ties to even.  The
+// quotient is taken as x * (1 / scale), which is off by less than 2^-23 of 127; where that leaves
+// doubt about the nearest integer (1 value in 10^4), the sign of x - (n + 1/2) scale decides, which
+// one fused multiply-add gives exactly.
+__device__ __forceinline__ int quantize_one(float x, float scale, float inv) {
+  const float t = x * inv;
+  float r = rintf(t);
+  if (fabsf(fabsf(t - r) - 0.5f) < 6e-5f) {
+    const float half = floorf(t) + 0.5f;
+    const float d = fmaf(-half, scale, x);
+    r = d > 0.f ? half + 0.5f : d < 0.f ? half - 0.5f : rintf(half);
+  }
+  return (int)fminf(fmaxf(r, -127.f), 127.f);
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(256)
+quantize_rows_kernel(const T* __restrict__ x, int64_t R, int K, int8_t* __restrict__ q, float* __restrict__ scale) {
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row >= R) return;
+  const int lane = threadIdx.x & 31;
+  const T* xr = x + row * K;
+  uint32_t top = 0;                                          // of the magnitudes' bits: NaN above infinity above all
+  for (int k = lane * V; k < K; k += 32 * V) {
+    float v[V];
+    if constexpr (V > 1) Vec16<T>::load(xr + k, v);
+    else v[0] = Elem<T>::to_f(xr[k]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  const float s = __fdiv_rn(__uint_as_float(top), 127.f);
+  if (lane == 0) scale[row] = s;
+  const bool zero = !(s > 0.f && s < __int_as_float(0x7f800000));    // all zero, or not finite: the scale says it
+  // rows of tiny values: both sides times 2^100, so that neither 1 / scale overflows nor the
+  // difference above leaves the range of fp32
+  const float up = s < 0x1p-100f ? 0x1p100f : 1.f;
+  const float su = s * up, inv = zero ? 0.f : __fdiv_rn(1.f, su);
+  for (int k = lane * V; k < K; k += 32 * V) {
+    float v[V];
+    if constexpr (V > 1) Vec16<T>::load(xr + k, v);
+    else v[0] = Elem<T>::to_f(xr[k]);
+    uint32_t w[(V + 3) / 4] = {};
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int n = zero ? 0 : quantize_one(v[i] * up, su, inv);
+      w[i >> 2] |= ((uint32_t)n & 0xffu) << (8 * (i & 3));
+    }
+    int8_t* d = q + row * K + k;
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
+    else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(d) = w[0];
+    else *d = (int8_t)w[0];
+  }
+}
+
+template <typename T>
+static int launch_quantize(const void* x, int64_t R, int K, void* q, float* scale, cudaStream_t st) {
+  constexpr int V = Vec16<T>::N;
+  const unsigned grid = (unsigned)((R + 7) / 8);
+  const bool wide = K % V == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & (V - 1)) == 0;
+  if (wide)
+    quantize_rows_kernel<T, V><<<grid, 256, 0, st>>>(static_cast<const T*>(x), R, K, static_cast<int8_t*>(q), scale);
+  else
+    quantize_rows_kernel<T, 1><<<grid, 256, 0, st>>>(static_cast<const T*>(x), R, K, static_cast<int8_t*>(q), scale);
+  MOLE_LAUNCH_OK();
+  return MOLE_OK;
+}
+
+static int check_sizes(int64_t R, int a, int b, int E) {
+  MOLE_REQUIRE(R >= 0 && R < (1ll << 31) - 65536, "rows=%lld", (long long)R);
+  MOLE_REQUIRE(a >= 1 && b >= 1 && a <= (1 << 21) && b <= (1 << 21), "widths %d, %d", a, b);
+  MOLE_REQUIRE(E >= 1 && E <= kMaxRaggedExperts, "E=%d (1..%d)", E, kMaxRaggedExperts);
+  return MOLE_OK;
+}
+static bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+}  // namespace mole
+
+using namespace mole;
+
+extern "C" int mole_grouped_mm(const void* x, const void* w, const int32_t* offsets, int64_t R,
+                               int32_t N, int32_t K, int32_t E, int32_t w_kn, int32_t dtype,
+                               void* out, void* stream) {
+  if (int rc = check_sizes(R, N, K, E)) return rc;
+  MOLE_REQUIRE(dtype == MOLE_F32 || dtype == MOLE_BF16, "dtype %d", dtype);
+  if (R == 0) return MOLE_OK;
+  MOLE_REQUIRE(x && w && offsets && out, "null pointer argument");
+  const size_t size = dtype == MOLE_F32 ? 4 : 2;
+  MOLE_REQUIRE(aligned_to(x, size) && aligned_to(w, size) && aligned_to(out, size) && aligned_to(offsets, 4), "a pointer is not aligned to its element");
+  RaggedRows a{};
+  a.x = x; a.w = w; a.offsets = offsets; a.out = out;
+  a.R = R; a.N = N; a.K = K; a.E = E; a.kn = w_kn != 0;
+  return ragged_rows_simt(dtype, a, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int mole_grouped_mm_wgrad(const void* a, const void* b, const int32_t* offsets, int64_t R,
+                                     int32_t P, int32_t Q, int32_t E, int32_t dtype, void* out,
+                                     void* stream) {
+  if (int rc = check_sizes(R, P, Q, E)) return rc;
+  MOLE_REQUIRE(dtype == MOLE_F32 || dtype == MOLE_BF16, "dtype %d", dtype);
+  MOLE_REQUIRE((a && b) || R == 0, "null pointer argument");
+  MOLE_REQUIRE(offsets && out, "null pointer argument");
+  const size_t size = dtype == MOLE_F32 ? 4 : 2;
+  MOLE_REQUIRE(aligned_to(a, size) && aligned_to(b, size) && aligned_to(out, size) && aligned_to(offsets, 4), "a pointer is not aligned to its element");
+  RaggedWgrad g{};
+  g.a = a; g.b = b; g.offsets = offsets; g.out = out;
+  g.R = R; g.P = P; g.Q = Q; g.E = E;
+  return ragged_wgrad_simt(dtype, g, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int mole_quantize_rows(const void* x, int64_t R, int32_t K, int32_t dtype, void* q,
+                                  float* scale, void* stream) {
+  MOLE_REQUIRE(R >= 0 && R < (1ll << 33), "rows=%lld", (long long)R);
+  MOLE_REQUIRE(K >= 1 && K <= (1 << 21), "K=%d", K);
+  MOLE_REQUIRE(dtype == MOLE_F32 || dtype == MOLE_BF16, "dtype %d", dtype);
+  if (R == 0) return MOLE_OK;
+  MOLE_REQUIRE(x && q && scale, "null pointer argument");
+  MOLE_REQUIRE(aligned_to(x, dtype == MOLE_F32 ? 4 : 2) && aligned_to(scale, 4), "a pointer is not aligned to its element");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == MOLE_F32 ? launch_quantize<float>(x, R, K, q, scale, st)
+                           : launch_quantize<__nv_bfloat16>(x, R, K, q, scale, st);
+}
+
+extern "C" int mole_grouped_mm_i8(const void* q, const float* q_scale, const void* w, const float* w_scale,
+                                  const int32_t* offsets, int64_t R, int32_t N, int32_t K, int32_t E,
+                                  int32_t out_dtype, void* out, void* stream) {
+  if (int rc = check_sizes(R, N, K, E)) return rc;
+  MOLE_REQUIRE(out_dtype == MOLE_F32 || out_dtype == MOLE_BF16, "dtype %d", out_dtype);
+  // |q w| <= 2^14: more terms could leave 32 bits
+  MOLE_REQUIRE(K < (1 << 17), "K=%d: sums of 2^17 and more products may leave 32 bits", K);
+  MOLE_REQUIRE(offsets || E == 1, "offsets may be null for one expert only");
+  if (R == 0) return MOLE_OK;
+  MOLE_REQUIRE(q && q_scale && w && w_scale && out, "null pointer argument");
+  MOLE_REQUIRE(aligned_to(out, out_dtype == MOLE_F32 ? 4 : 2) && aligned_to(q_scale, 4) && aligned_to(w_scale, 4) && aligned_to(offsets, 4), "a pointer is not aligned to its element");
+  RaggedRows a{};
+  a.x = q; a.w = w; a.offsets = offsets; a.x_scale = q_scale; a.w_scale = w_scale; a.out = out;
+  a.R = R; a.N = N; a.K = K; a.E = E;
+  return ragged_rows_simt_i8(out_dtype, a, static_cast<cudaStream_t>(stream));
+}

@@ -1,0 +1,94 @@
+// Products over rows packed by expert: interface between the C entries (ragged.cu) and the kernels.
+//
+// Expert e owns the rows [offsets[e], offsets[e + 1]) of the packed matrices; the offsets live on
+// the device and are never read by the host.  Rows before offsets[0] and from offsets[E] on belong
+// to nobody: products write zeros there.  Offsets are clamped on the device to 0 <= o[0] <= ... <= R,
+// so a bad array costs a wrong result and never an access out of range.
+#pragma once
+#include "common.cuh"
+
+namespace mole {
+
+struct RaggedRows {         // out[r, n] = sum_k x[r, k] w_e(n, k)
+  const void* x;            // [R, K]
+  const void* w;            // [E, N, K] (kn = 0) or [E, K, N] (kn = 1)
+  const int32_t* offsets;   // [E + 1], or null: one expert, all rows
+  const float* x_scale;     // 8-bit integers: scale of row r,
+  const float* w_scale;     //                 scale of channel (e, n)
+  void* out;                // [R, N]
+  int64_t R;
+  int N, K, E, kn;
+};
+struct RaggedWgrad {        // out[e, p, q] = sum over the rows r of e of a[r, p] b[r, q]
+  const void* a;            // [R, P]
+  const void* b;            // [R, Q]
+  const int32_t* offsets;
+  void* out;                // [E, P, Q]
+  int64_t R;
+  int P, Q, E;
+};
+
+int ragged_rows_simt(int dtype, const RaggedRows& a, cudaStream_t st);
+int ragged_rows_simt_i8(int out_dtype, const RaggedRows& a, cudaStream_t st);
+int ragged_wgrad_simt(int dtype, const RaggedWgrad& a, cudaStream_t st);
+
+constexpr int kMaxRaggedExperts = 256;
+// Spans of rows: 0 = the rows before the first expert, 1 .. E = the experts, E + 1 = the rows behind
+// the last.  row0[i] .. row0[i + 1] is span i, tile0[i] the tiles of `unit` rows before it.
+struct RaggedSpans {
+  int row0[kMaxRaggedExperts + 3];
+  int tile0[kMaxRaggedExperts + 3];
+};
+
+// By one whole warp; the caller synchronises the block afterwards.
+__device__ __forceinline__ void load_spans(RaggedSpans& s, const int32_t* offsets, int E, int R, int unit) {
+  const int lane = threadIdx.x & 31;
+  const int n = E + 1;                               // offsets
+  const int per = (n + 31) / 32;
+  const int i0 = lane * per, i1 = min(n, i0 + per);
+  int run = 0;
+  for (int i = i0; i < i1; ++i) {
+    int o = offsets ? offsets[i] : (i == 0 ? 0 : R);
+    run = max(run, min(max(o, 0), R));
+    s.row0[i + 1] = run;
+  }
+  int before = run;                                  // running maximum over the lanes, then of those before
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, before, d);
+    if (lane >= d) before = max(before, v);
+  }
+  before = __shfl_up_sync(0xffffffffu, before, 1);
+  if (lane == 0) before = 0;
+  for (int i = i0; i < i1; ++i) s.row0[i + 1] = max(s.row0[i + 1], before);
+  if (lane == 0) { s.row0[0] = 0; s.row0[E + 2] = R; }
+  __syncwarp();
+  // tiles of the E + 2 spans
+  const int ns = E + 2, pers = (ns + 31) / 32;
+  const int j0 = lane * pers, j1 = min(ns, j0 + pers);
+  int sum = 0;
+  for (int j = j0; j < j1; ++j) sum += (s.row0[j + 1] - s.row0[j] + unit - 1) / unit;
+  int incl = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += v;
+  }
+  int at = incl - sum;
+  for (int j = j0; j < j1; ++j) {
+    s.tile0[j] = at;
+    at += (s.row0[j + 1] - s.row0[j] + unit - 1) / unit;
+  }
+  if (lane == 31) s.tile0[ns] = incl;
+}
+// the span that holds tile t (t < tile0[E + 2]): the last one that starts at or before it
+__device__ __forceinline__ int span_of(const RaggedSpans& s, int E, int t) {
+  int lo = 0, hi = E + 2;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s.tile0[mid] <= t) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+}  // namespace mole

@@ -312,6 +312,113 @@ def ffn_bwd_peer(desc: FfnDesc, counts, dout, x, x1, h, w1, w2, dx1, peer, gw1, 
                                 ws.numel(), _stream()))
 
 
+# ---- products over rows packed by expert --------------------------------------------------------
+def _check_offsets(offsets: torch.Tensor, E: int) -> None:
+    if offsets.dtype != torch.int32 or offsets.shape != (E + 1,):
+        raise ValueError(f"offsets must be int32 [{E + 1}]")
+
+
+def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, w_kn: bool = False,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``out[r] = x[r] @ w[e].T`` (``w`` ``[E, N, K]``), or ``x[r] @ w[e]`` with ``w_kn`` (``w``
+    ``[E, K, N]``), for the rows ``offsets[e] <= r < offsets[e + 1]`` of every expert.  ``offsets``
+    (int32 ``[E + 1]``, ``RoutePlan.offsets``) stays on the device; rows of no expert become zeros."""
+    if x.dim() != 2 or w.dim() != 3:
+        raise ValueError("grouped_mm takes x [R, K] and w [E, N, K] or [E, K, N]")
+    E, N, K = w.shape[0], w.shape[2 if w_kn else 1], w.shape[1 if w_kn else 2]
+    if x.shape[1] != K:
+        raise ValueError(f"x has width {x.shape[1]}, the weights take {K}")
+    if w.dtype != x.dtype:
+        raise TypeError("x and w must have one dtype")
+    _check_offsets(offsets, E)
+    if out is None:
+        out = torch.empty(x.shape[0], N, dtype=x.dtype, device=x.device)
+    elif out.shape != (x.shape[0], N) or out.dtype != x.dtype:
+        raise ValueError(f"out must be {x.dtype} [{x.shape[0]}, {N}]")
+    with _on_device_of(x, w, offsets, out):
+        check(lib.mole_grouped_mm(_ptr(x), _ptr(w), _ptr(offsets), x.shape[0], N, K, E, int(w_kn), _dt(x),
+                                  _ptr(out), _stream()))
+    return out
+
+
+def grouped_mm_wgrad(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``out[e] = a_e.T @ b_e`` over the rows of every expert: ``[E, P, Q]`` from ``a [R, P]`` and
+    ``b [R, Q]``; zeros for an expert without rows."""
+    if a.dim() != 2 or b.dim() != 2 or a.shape[0] != b.shape[0]:
+        raise ValueError("grouped_mm_wgrad takes a [R, P] and b [R, Q]")
+    if a.dtype != b.dtype:
+        raise TypeError("a and b must have one dtype")
+    E, P, Q = offsets.numel() - 1, a.shape[1], b.shape[1]
+    _check_offsets(offsets, E)
+    if out is None:
+        out = torch.empty(E, P, Q, dtype=a.dtype, device=a.device)
+    elif out.shape != (E, P, Q) or out.dtype != a.dtype:
+        raise ValueError(f"out must be {a.dtype} [{E}, {P}, {Q}]")
+    with _on_device_of(a, b, offsets, out):
+        check(lib.mole_grouped_mm_wgrad(_ptr(a), _ptr(b), _ptr(offsets), a.shape[0], P, Q, E, _dt(a),
+                                        _ptr(out), _stream()))
+    return out
+
+
+def quantize_rows(x: torch.Tensor):
+    """``(q int8, scale float32)``: every row (last dimension) of ``x`` in 8-bit integers with one
+    scale, ``q = round(x / scale)``, ``scale = max|row| / 127``.  Used for tokens (``[R, K]``) and, once, for
+    weights ``[E, N, K]``, whose rows are the output channels."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("quantize_rows needs rows of at least one element")
+    K = x.shape[-1]
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    with _on_device_of(x):
+        check(lib.mole_quantize_rows(_ptr(x), scale.numel(), K, _dt(x), _ptr(q), _ptr(scale), _stream()))
+    return q, scale
+
+
+def _mm_int8(q, q_scale, w, w_scale, offsets, E, N, K, out_dtype, out):
+    if q.dtype != torch.int8 or w.dtype != torch.int8:
+        raise TypeError("the operands must be int8")
+    if q.dim() != 2 or q.shape[1] != K:
+        raise ValueError(f"q must be [R, {K}]")
+    R = q.shape[0]
+    if q_scale.dtype != torch.float32 or q_scale.shape != (R,):
+        raise ValueError(f"q_scale must be float32 [{R}]")
+    if w_scale.dtype != torch.float32 or w_scale.shape != w.shape[:-1]:
+        raise ValueError(f"w_scale must be float32 {list(w.shape[:-1])}")
+    if out_dtype not in _DTYPES:
+        raise TypeError(f"unsupported dtype {out_dtype}; the kernels cover float32 and bfloat16")
+    if out is None:
+        out = torch.empty(R, N, dtype=out_dtype, device=q.device)
+    elif out.shape != (R, N) or out.dtype != out_dtype:
+        raise ValueError(f"out must be {out_dtype} [{R}, {N}]")
+    with _on_device_of(q, q_scale, w, w_scale, offsets, out):
+        check(lib.mole_grouped_mm_i8(_ptr(q), _ptr(q_scale), _ptr(w), _ptr(w_scale), _ptr(offsets), R, N, K, E,
+                                     _DTYPES[out_dtype], _ptr(out), _stream()))
+    return out
+
+
+def grouped_mm_int8(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                    offsets: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``grouped_mm`` of 8-bit integers: ``out[r, n] = (q[r] . w[e, n]) * q_scale[r] * w_scale[e, n]`` with
+    ``q [R, K]``, ``w [E, N, K]`` int8 (``quantize_rows`` of the tokens and of the weights), the sum of
+    products exact."""
+    if w.dim() != 3:
+        raise ValueError("grouped_mm_int8 takes w [E, N, K]")
+    E, N, K = w.shape
+    _check_offsets(offsets, E)
+    return _mm_int8(q, q_scale, w, w_scale, offsets, E, N, K, out_dtype, out)
+
+
+def mm_int8(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+            out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The same product with one weight matrix ``w [N, K]`` for all rows."""
+    if w.dim() != 2:
+        raise ValueError("mm_int8 takes w [N, K]")
+    N, K = w.shape
+    return _mm_int8(q, q_scale, w, w_scale, None, 1, N, K, out_dtype, out)
+
+
 # ---- one Adam step over many tensors ---------------------------------------------------------
 ADAM_BLOCK = 256      # elements of an 8-bit moment that share one scale
 
