@@ -18,13 +18,12 @@
 //
 // Every wait on an mbarrier is bounded: when it runs out the kernel records a code in the
 // library's fault word, stops waiting for the rest of its run, still frees its TMEM and exits.
-#include <cuda.h>
-
 #include <mutex>
 #include <type_traits>
 #include <unordered_map>
 
 #include "gemm.cuh"
+#include "tc_ptx.cuh"
 
 namespace mole {
 
@@ -39,133 +38,6 @@ constexpr int kEpiWarps = 16;
 constexpr int kThreads = 32 * (2 + kEpiWarps);
 
 enum TcMode : int { TC_ROWS = 0, TC_WGRAD = 1 };
-
-// ---- PTX wrappers ---------------------------------------------------------------------
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n.reg .pred p;\n"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-      "selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ uint64_t globaltimer_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-// Bounded wait; false when it gave up.  `abort_flag` lives in shared memory: once any wait of
-// this CTA has run out, later waits return false at once.  A role that sees false leaves its
-// work loop: it issues no further TMA load or MMA and stores nothing more, so an output that
-// the accumulator never reached is not written (the fault word tells the host that the step's
-// results are not to be used).
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                          int32_t* fault, int code) {
-  if (mbar_try_wait(bar, parity)) return true;
-  if (*abort_flag) return false;
-  const uint64_t t0 = globaltimer_ns();
-  uint32_t polls = 0;
-  while (!mbar_try_wait(bar, parity)) {
-    if ((++polls & 0x3ff) == 0) {
-      if (*abort_flag) return false;
-      if (globaltimer_ns() - t0 > 2000000000ull) {     // 2 s
-        *abort_flag = 1;
-        atomicCAS(fault, 0, code);
-        return false;
-      }
-    }
-  }
-  return true;
-}
-// After an abort: what this CTA has already issued (TMA loads into its shared memory, MMAs that
-// read it) gets a bounded time to land before the CTA frees its TMEM and exits.
-__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity, uint64_t deadline_ns) {
-  uint32_t polls = 0;
-  while (!mbar_try_wait(bar, parity))
-    if ((++polls & 0xff) == 0 && globaltimer_ns() > deadline_ns) return;
-}
-// Producer side of the drain: stage s of a ring of `stages` has been armed
-// n_s = issued / stages + (s < issued % stages) times; the parity of its last phase is (n_s - 1) & 1.
-__device__ __forceinline__ void drain_loads(uint32_t full0, int stages, uint32_t issued) {
-  const uint64_t deadline = globaltimer_ns() + 200000000ull;      // 0.2 s for all of them
-  for (int s = 0; s < stages; ++s) {
-    const uint32_t n_s = issued / stages + ((uint32_t)s < issued % stages ? 1u : 0u);
-    if (n_s > 0) mbar_drain(full0 + 8 * s, (n_s - 1) & 1u, deadline);
-  }
-}
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
-                                            int c0, int c1) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
-}
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
-                                            int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-      ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
-}
-__device__ __forceinline__ void tcgen05_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tcgen05_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tcgen05_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-               ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tcgen05_mma_bf16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
-                                                 uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld_wait() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-// Shared-memory matrix descriptor, 128-byte swizzle, bf16 (layouts as documented for UMMA):
-//   K-major  : rows of 128 B (64 K elements), 8-row groups 1024 B apart (SBO); LBO unused
-//   MN-major : 64 MN elements (128 B) contiguous per K row, 8 K rows per 1024-byte group (SBO),
-//              next 64 MN elements `lbo_bytes` further (LBO)
-__device__ __forceinline__ uint64_t make_desc(uint32_t saddr, uint32_t lbo_bytes,
-                                              uint32_t sbo_bytes) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr & 0x3ffff) >> 4);
-  d |= (uint64_t)((lbo_bytes >> 4) & 0x3fff) << 16;
-  d |= (uint64_t)((sbo_bytes >> 4) & 0x3fff) << 32;
-  d |= (uint64_t)1 << 46;      // descriptor version of sm_100
-  d |= (uint64_t)2 << 61;      // SWIZZLE_128B
-  return d;
-}
 
 // 32 bf16 = 64 bytes per thread, moved as two 32-byte vectors so that every request covers a
 // whole 32-byte sector
@@ -435,16 +307,6 @@ __device__ __forceinline__ uint32_t act_bwd_pair(float v0, float v1, uint32_t xw
   float o0, o1;
   f2_unpack(f2_mul(f2_pack(v0, v1), d), o0, o1);
   return pack_bf16(o0, o1);
-}
-
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
 }
 
 // The epilogue works in steps of 16 columns: one tcgen05.ld of 16 accumulator columns, the fused
@@ -1001,7 +863,6 @@ tc_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
 // Barriers: TMA loads of both CTAs complete on the even CTA's "full" barrier (.cta_group::2
 // form, no multicast); stage release and accumulator-ready are tcgen05.commit arrivals multicast
 // to both CTAs' barriers; the odd CTA's epilogue releases the accumulator with a remote arrive.
-constexpr uint32_t kPeerMask = 0xFEFFFFFFu;     // clears the CTA-rank bit of a shared::cluster address
 constexpr int kBN2 = 256;
 template <int KR> struct Pair2 {
   static constexpr uint32_t kBoxBytes = 128 * KR;
@@ -1009,43 +870,6 @@ template <int KR> struct Pair2 {
   static constexpr uint32_t kBHalfBytes = (kBN2 / 2) * KR * 2;
   static constexpr uint32_t kStageBytes = kABytes + kBHalfBytes;
 };
-
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ void tma2_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
-                                             int c0, int c1) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-      ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
-}
-__device__ __forceinline__ void tma2_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
-                                             int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-      ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2) : "memory");
-}
-__device__ __forceinline__ void tcgen05_commit2(uint32_t bar) {   // arrives in both CTAs of the pair
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-      ::"r"(bar), "h"((uint16_t)3) : "memory");
-}
-__device__ __forceinline__ void tcgen05_mma2_bf16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
-                                                  uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}"
-      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
-}
 
 struct PairItem {
   int valid;
@@ -1397,8 +1221,6 @@ struct MapKeyHash {
     return (size_t)(h ^ (uint64_t)k.rank);
   }
 };
-static int encode_map(CUtensorMap* m, const void* base, int rank, const uint64_t* dims,
-                      const uint32_t* box);
 static int make_map(CUtensorMap* m, const void* base, int rank, const uint64_t* dims,
                     const uint32_t* box) {
   static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
@@ -1410,20 +1232,19 @@ static int make_map(CUtensorMap* m, const void* base, int rank, const uint64_t* 
   std::lock_guard<std::mutex> lock(mu);
   auto it = cache.find(key);
   if (it != cache.end()) { *m = it->second; return MOLE_OK; }
-  if (int rc = encode_map(m, base, rank, dims, box)) return rc;
+  if (int rc = encode_map(m, base, rank, dims, box, 2)) return rc;
   if (cache.size() > 4096) cache.clear();
   cache.emplace(key, *m);
   return MOLE_OK;
 }
 
-// bf16 tensor, innermost dimension contiguous, 128-byte swizzle, box inner extent 64 elements
-static int encode_map(CUtensorMap* m, const void* base, int rank, const uint64_t* dims,
-                      const uint32_t* box) {
+int encode_map(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint32_t* box,
+               int elem) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(MOLE_ERR_CUDA, "cuTensorMapEncodeTiled entry point not found");
   cuuint64_t gdim[3], gstride[2];
   cuuint32_t bdim[3], estr[3] = {1, 1, 1};
-  uint64_t stride = 2;
+  uint64_t stride = (uint64_t)elem;
   for (int i = 0; i < rank; ++i) {
     gdim[i] = dims[i];
     bdim[i] = box[i];
@@ -1431,7 +1252,7 @@ static int encode_map(CUtensorMap* m, const void* base, int rank, const uint64_t
     if (i < rank - 1) gstride[i] = stride;
   }
   MOLE_REQUIRE((reinterpret_cast<uintptr_t>(base) & 15) == 0, "tensor base %p not 16-byte aligned", base);
-  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), gdim,
+  const CUresult r = fn(m, elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), gdim,
                         gstride, bdim, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
