@@ -1252,10 +1252,18 @@ int encode_map(CUtensorMap* m, const void* base, int rank, const uint64_t* dims,
     if (i < rank - 1) gstride[i] = stride;
   }
   MOLE_REQUIRE((reinterpret_cast<uintptr_t>(base) & 15) == 0, "tensor base %p not 16-byte aligned", base);
-  const CUresult r = fn(m, elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), gdim,
-                        gstride, bdim, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return fn(m, elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
+              const_cast<void*>(base), gdim, gstride, bdim, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {      // a thread's first CUDA call (autograd's): no context is current yet
+    int dev = 0;
+    MOLE_CUDA_OK(cudaGetDevice(&dev));
+    MOLE_CUDA_OK(cudaSetDevice(dev));
+    r = encode();
+  }
   if (r != CUDA_SUCCESS) return fail(MOLE_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
   return MOLE_OK;
 }

@@ -97,6 +97,7 @@ extern "C" int mole_grouped_mm(const void* x, const void* w, const int32_t* offs
   RaggedRows a{};
   a.x = x; a.w = w; a.offsets = offsets; a.out = out;
   a.R = R; a.N = N; a.K = K; a.E = E; a.kn = w_kn != 0;
+  if (dtype == MOLE_BF16 && ragged_rows_tc_takes(2, a)) return ragged_rows_tc(2, dtype, a, static_cast<cudaStream_t>(stream));
   return ragged_rows_simt(dtype, a, static_cast<cudaStream_t>(stream));
 }
 
@@ -112,6 +113,7 @@ extern "C" int mole_grouped_mm_wgrad(const void* a, const void* b, const int32_t
   RaggedWgrad g{};
   g.a = a; g.b = b; g.offsets = offsets; g.out = out;
   g.R = R; g.P = P; g.Q = Q; g.E = E;
+  if (dtype == MOLE_BF16 && ragged_wgrad_tc_takes(g)) return ragged_wgrad_tc(g, static_cast<cudaStream_t>(stream));
   return ragged_wgrad_simt(dtype, g, static_cast<cudaStream_t>(stream));
 }
 
@@ -142,5 +144,6 @@ extern "C" int mole_grouped_mm_i8(const void* q, const float* q_scale, const voi
   RaggedRows a{};
   a.x = q; a.w = w; a.offsets = offsets; a.x_scale = q_scale; a.w_scale = w_scale; a.out = out;
   a.R = R; a.N = N; a.K = K; a.E = E;
+  if (ragged_rows_tc_takes(1, a)) return ragged_rows_tc(1, out_dtype, a, static_cast<cudaStream_t>(stream));
   return ragged_rows_simt_i8(out_dtype, a, static_cast<cudaStream_t>(stream));
 }

@@ -1,0 +1,753 @@
+// Products over rows packed by expert on the sm_100a tensor cores: bf16 with fp32 sums and 8-bit
+// integers with 32-bit sums (tcgen05.mma, cta_group::2, accumulators in TMEM, operands by TMA).
+//
+// Rows product.  The weights are the M side: a pair of CTAs takes 256 output features of one expert,
+// 128 each, and a panel of up to 256 of its rows as the N side, in steps of 16 (32 for integers), so
+// that ragged row counts cost their own size and not the next multiple of 128 or 256.  A stage of
+// the ring is 128 bytes of the reduction: this CTA's 128 features (16 KB) and its half of the panel's
+// rows.  Two accumulators of 256 columns: one panel's epilogue runs under the next one's main loop.
+// Neighbouring rows that a panel's last step reads belong to other experts: each row is a column of
+// the accumulator of its own, and such columns are not stored.
+//
+// Weight gradient.  out_e = a_e^T b_e: 256 x 256 of an expert's matrix per pair, the reduction runs
+// over its rows, 64 per stage.  The last 16-row step of an expert may reach into rows of others,
+// which must not enter the sum, not even as 0 times NaN: a warp per CTA (the "fixer") writes zeros
+// over them in shared memory, in both operands, before that stage is handed to the tensor cores.
+// There are no padding rows in memory to do without it, and 16 rows are all that is wasted.
+//
+// Every wait is bounded: a wait that runs out leaves a code in the fault word, the CTA's other roles
+// stop at their next wait, copies in flight get time to land, the TMEM is freed.
+#include <type_traits>
+
+#include "ragged.cuh"
+#include "tc_ptx.cuh"
+
+namespace mole {
+
+constexpr int kREpiWarps = 16;
+constexpr int kRThreads = 32 * (4 + kREpiWarps);         // producer, issuer, fixer, spare, epilogue
+constexpr uint32_t kRABytes = 128 * 128;                 // 128 features x 128 bytes of the reduction
+constexpr int kRMaxStages = 12;
+constexpr uint32_t kRStripBytes = 1024;                  // per epilogue warp
+
+struct RowsMaps {
+  CUtensorMap w;        // K-major: 128 B x 128 features; N-major: 64 features x 64 of the reduction
+  CUtensorMap x[4];     // 128 B x {64, 32, 16, 8} rows
+};
+struct RowsParams {
+  const int32_t* offsets;
+  const float* x_scale;
+  const float* w_scale;
+  void* out;
+  int32_t* fault;
+  int R, N, E;
+  int nkb;              // stages of the reduction
+  int wide;             // rows of out are multiples of 16 bytes, its base too
+  int stages;
+  uint32_t stage_bytes;
+};
+
+// The experts' spans without tiles, in the order of falling row counts: the round-robin deal of the
+// items gives every pair its share of large and of small ones.
+struct RowsOrder {
+  int row0[kMaxRaggedExperts + 3];       // as RaggedSpans
+  int tile0[kMaxRaggedExperts + 3];
+  int start[kMaxRaggedExperts + 1];      // panels before the i-th expert of the order
+  uint8_t order[kMaxRaggedExperts];
+};
+struct RowsItem {
+  int valid;
+  int e, f0;             // expert, first of the pair's 256 features
+  int row0, rows, n;     // panel: first row, rows, columns of the accumulator
+};
+
+template <int STEP>
+__device__ __forceinline__ RowsItem rows_item(const RowsOrder& o, int E, int nb, int item) {
+  RowsItem w;
+  w.valid = 0;
+  if (item >= o.start[E] * nb) return w;
+  int lo = 0, hi = E;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (o.start[mid] * nb <= item) lo = mid; else hi = mid;
+  }
+  const int np = o.start[lo + 1] - o.start[lo];
+  const int local = item - o.start[lo] * nb;
+  const int pan = local % np;              // panels of a feature block are neighbours: they share weights through L2
+  const int e = o.order[lo];
+  const int b = o.row0[e + 1], cnt = o.row0[e + 2] - b;
+  const int per = ((cnt + np - 1) / np + STEP - 1) / STEP * STEP;
+  w.valid = 1;
+  w.e = e;
+  w.f0 = local / np * 256;
+  w.row0 = b + pan * per;
+  w.rows = min(per, cnt - pan * per);      // may be <= 0 for a last panel: nothing to do
+  w.n = (max(w.rows, 0) + STEP - 1) / STEP * STEP;
+  return w;
+}
+
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                                  int32_t* fault, int code) {
+  if (mbar_try_wait_cluster(bar, parity)) return true;
+  if (!mbar_wait(bar, parity, abort_flag, fault, code)) return false;
+  return mbar_try_wait_cluster(bar, parity) || true;      // completed: this one orders what the peer wrote
+}
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ void fence_async_proxy() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ bool warp_all_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* fault, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, fault, code));
+}
+// after an abort: loads already issued take microseconds to land; they get 20 ms
+__device__ __forceinline__ void settle() {
+  const uint64_t t0 = globaltimer_ns();
+  while (globaltimer_ns() - t0 < 20000000ull) __nanosleep(1000);
+}
+__device__ __forceinline__ void tcgen05_mma2_i8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                                uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}"
+      ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ uint32_t two_bf16(float lo, float hi) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// Zeros into the rows that belong to nobody, by the epilogue warps of all CTAs
+template <typename TO>
+__device__ __forceinline__ void zero_rows(TO* out, int r0, int r1, int N, int worker, int workers, int lane) {
+  for (int r = r0 + worker; r < r1; r += workers)
+    for (int n = lane; n < N; n += 32) out[(int64_t)r * N + n] = Elem<TO>::from_f(0.f);
+}
+
+// One chunk of 16 rows x 32 features of a warp, bf16: turned round through a 1 KB strip so that a
+// lane stores eight neighbouring features of two rows.  Word (rp, l) of the strip holds rows 2 rp
+// and 2 rp + 1 of feature l, at rp * 32 + (l ^ 4 (rp & 1)): no bank conflicts on either side.
+__device__ __forceinline__ void store_chunk(__nv_bfloat16* out, const float (&v)[16], uint32_t* strip, int row, int rows_left,
+                                            int f_warp, int N, int lane) {
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) strip[32 * i + (lane ^ ((i & 1) << 2))] = two_bf16(v[2 * i], v[2 * i + 1]);
+  __syncwarp();
+  const int rp = lane >> 2, g = lane & 3;
+  const uint4* s4 = reinterpret_cast<const uint4*>(strip);
+  const uint4 lo = s4[rp * 8 + 2 * g + (rp & 1)], hi = s4[rp * 8 + 2 * g + 1 - (rp & 1)];
+  const int f = f_warp + 8 * g;
+  if (f < N) {
+    __nv_bfloat16* d = out + (int64_t)(row + 2 * rp) * N + f;
+    if (2 * rp < rows_left)
+      *reinterpret_cast<uint4*>(d) = make_uint4(__byte_perm(lo.x, lo.y, 0x5410), __byte_perm(lo.z, lo.w, 0x5410),
+                                                __byte_perm(hi.x, hi.y, 0x5410), __byte_perm(hi.z, hi.w, 0x5410));
+    if (2 * rp + 1 < rows_left)
+      *reinterpret_cast<uint4*>(d + N) = make_uint4(__byte_perm(lo.x, lo.y, 0x7632), __byte_perm(lo.z, lo.w, 0x7632),
+                                                    __byte_perm(hi.x, hi.y, 0x7632), __byte_perm(hi.z, hi.w, 0x7632));
+  }
+}
+
+template <bool I8, bool KN, typename TO>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kRThreads, 1)
+ragged_rows_tc_kernel(const __grid_constant__ RowsMaps maps, const __grid_constant__ RowsParams p) {
+  static_assert(!(I8 && KN), "integers are read K-major");
+  constexpr int STEP = I8 ? 32 : 16;             // columns of the accumulator come in these steps
+  constexpr int KB = I8 ? 128 : 64;              // elements of the reduction per stage
+  constexpr uint32_t kIdesc = ((I8 ? 2u : 1u) << 4) | (1u << 7) | (1u << 10) | ((KN ? 1u : 0u) << 15) |
+                              ((uint32_t)(256 >> 4) << 24);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  __shared__ __align__(8) uint64_t bars[2 * kRMaxStages + 5];
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int abort_flag_s;
+  __shared__ RowsOrder ord;
+  __shared__ __align__(16) uint32_t strips[kREpiWarps][kRStripBytes / 4];
+  volatile int* abort_flag = &abort_flag_s;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[kRMaxStages]);
+  const uint32_t tfull0 = smem_u32(&bars[2 * kRMaxStages]), tempty0 = smem_u32(&bars[2 * kRMaxStages + 2]);
+  const uint32_t drain0 = smem_u32(&bars[2 * kRMaxStages + 4]);
+  const uint32_t smem_base = smem_u32(smem);
+  const int cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
+  const int E = p.E, nb = (p.N + 255) / 256;
+
+  if (warp == 0) load_spans(*reinterpret_cast<RaggedSpans*>(&ord), p.offsets, E, p.R, 256);
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&tmem_base_s)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  if (threadIdx.x == 64) {
+    abort_flag_s = 0;
+    mbar_init(drain0, 1);
+    for (int s = 0; s < kRMaxStages; ++s) {
+      mbar_init(full0 + 8 * s, 1);                  // the even CTA's arrive.expect_tx
+      mbar_init(empty0 + 8 * s, 1);                 // a commit that arrives in both CTAs
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull0 + 8 * a, 1);
+      mbar_init(tempty0 + 8 * a, 2 * kREpiWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += kRThreads) {
+    const int mine = ord.row0[e + 2] - ord.row0[e + 1];
+    int rk = 0;
+    for (int o = 0; o < E; ++o) {
+      const int other = ord.row0[o + 2] - ord.row0[o + 1];
+      rk += (other > mine) || (other == mine && o < e);
+    }
+    ord.order[rk] = (uint8_t)e;
+  }
+  __syncthreads();
+  if (warp == 0) {                                  // panels before the i-th expert of the order
+    int base = 0;
+    for (int i0 = 0; i0 < E; i0 += 32) {
+      const int i = i0 + lane;
+      int v = 0;
+      if (i < E) { const int e = ord.order[i]; v = ord.tile0[e + 2] - ord.tile0[e + 1]; }
+      int incl = v;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += u;
+      }
+      if (i < E) ord.start[i] = base + incl - v;
+      base += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) ord.start[E] = base;
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();                               // barriers initialised, TMEM addresses there, in both CTAs
+  tcgen05_fence_after();
+  const uint32_t tmem_base = tmem_base_s;
+
+  if (warp == 0) {
+    // ---- TMA producer (both CTAs; every box has its own lane) ----
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int item = cluster_id; ok; item += n_clusters) {
+      const RowsItem w = rows_item<STEP>(ord, E, nb, item);
+      if (!w.valid) break;
+      if (w.n == 0) continue;
+      const int h = w.n >> 1;                       // rows that this CTA stages
+      const uint32_t tx = 2u * (kRABytes + (uint32_t)h * 128u);
+      const int f0 = w.f0 + 128 * (int)rank;
+      int kind = -1, off = 0;                       // lanes 2..6: the panel's rows in boxes of 64, 64, 32, 16, 8
+      {
+        const int n64 = h >> 6, rem = h & 63;
+        if (lane == 2 || lane == 3) { if (lane - 2 < n64) { kind = 0; off = 64 * (lane - 2); } }
+        else if (lane == 4) { if (rem & 32) { kind = 1; off = 64 * n64; } }
+        else if (lane == 5) { if (rem & 16) { kind = 2; off = 64 * n64 + (rem & 32); } }
+        else if (lane == 6) { if (rem & 8) { kind = 3; off = 64 * n64 + (rem & 48); } }
+      }
+      const int srow = w.row0 + h * (int)rank + off;
+      for (int kb = 0; kb < p.nkb; ++kb) {
+        ok = warp_all_wait(empty0 + 8 * stage, phase ^ 1, abort_flag, p.fault, 61);
+        if (!ok) break;
+        const uint32_t bar = (full0 + 8 * stage) & kPeerMask;      // the even CTA's
+        const uint32_t sa = smem_base + stage * p.stage_bytes, sb = sa + kRABytes;
+        if (rank == 0 && lane == 0) mbar_expect_tx(full0 + 8 * stage, tx);
+        if (KN) {
+          if (lane < 2) tma2_load_3d(sa + lane * (kRABytes / 2), &maps.w, bar, f0 + 64 * lane, kb * KB, w.e);
+        } else {
+          if (lane == 0) tma2_load_3d(sa, &maps.w, bar, kb * KB, f0, w.e);
+        }
+        if (kind >= 0) tma2_load_2d(sb + off * 128, &maps.x[kind], bar, kb * KB, srow);
+        if (++stage == p.stages) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    // ---- MMA issuer (even CTA) ----
+    if (lane == 0 && rank == 0) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int item = cluster_id; ok; item += n_clusters) {
+        const RowsItem w = rows_item<STEP>(ord, E, nb, item);
+        if (!w.valid) break;
+        if (w.n == 0) continue;
+        if (!(ok = mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag, p.fault, 62))) break;
+        tcgen05_fence_after();
+        const uint32_t d_tmem = tmem_base + 256 * acc;
+        const uint32_t idesc = kIdesc | ((uint32_t)(w.n >> 3) << 17);
+        for (int kb = 0; kb < p.nkb; ++kb) {
+          if (!(ok = mbar_wait(full0 + 8 * stage, phase, abort_flag, p.fault, 63))) break;
+          tcgen05_fence_after();
+          const uint32_t sa = smem_base + stage * p.stage_bytes, sb = sa + kRABytes;
+#pragma unroll
+          for (int ks = 0; ks < 4; ++ks) {          // 32 bytes of the reduction each
+            const uint64_t ad = KN ? make_desc(sa + ks * (16 * 128), kRABytes / 2, 1024) : make_desc(sa + ks * 32, 16, 1024);
+            const uint64_t bd = make_desc(sb + ks * 32, 16, 1024);
+            if (I8) tcgen05_mma2_i8(d_tmem, ad, bd, idesc, (kb | ks) ? 1u : 0u);
+            else tcgen05_mma2_bf16(d_tmem, ad, bd, idesc, (kb | ks) ? 1u : 0u);
+          }
+          tcgen05_commit2(empty0 + 8 * stage);
+          if (++stage == p.stages) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        tcgen05_commit2(tfull0 + 8 * acc);
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      }
+      if (*abort_flag) {
+        tcgen05_commit2(drain0);
+        mbar_drain(drain0, 0, globaltimer_ns() + 200000000ull);
+      }
+    }
+  } else if (warp >= 4) {
+    // ---- epilogue (both CTAs): warp -> 32 features (the TMEM lanes it may read), every fourth chunk of 16 rows ----
+    const int quarter = warp & 3, grp = (warp - 4) >> 2;
+    uint32_t* strip = strips[warp - 4];
+    TO* out = static_cast<TO*>(p.out);
+    {
+      const int worker = blockIdx.x * kREpiWarps + warp - 4, workers = gridDim.x * kREpiWarps;
+      zero_rows(out, 0, ord.row0[1], p.N, worker, workers, lane);
+      zero_rows(out, ord.row0[E + 1], p.R, p.N, worker, workers, lane);
+    }
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int item = cluster_id;; item += n_clusters) {
+      const RowsItem w = rows_item<STEP>(ord, E, nb, item);
+      if (!w.valid) break;
+      if (w.n == 0) continue;
+      const int f_warp = w.f0 + 128 * (int)rank + 32 * quarter, f = f_warp + lane;
+      float ws = 0.f;
+      if (I8 && f < p.N) ws = p.w_scale[(int64_t)w.e * p.N + f];
+      if (!warp_all_wait(tfull0 + 8 * acc, acc_phase, abort_flag, p.fault, 64)) break;
+      tcgen05_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + 256 * acc;
+      for (int c = grp * 16; c < w.rows; c += 64) {
+        uint32_t r[16];
+        tmem_ld16(taddr + c, r);
+        tmem_ld_wait();
+        const int left = w.rows - c;                // rows of the chunk that exist: 1 .. 16 and more
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if (I8) {
+            const float xs = p.x_scale[w.row0 + c + min(i, left - 1)];
+            v[i] = __fmul_rn(__fmul_rn((float)(int)r[i], xs), ws);
+          } else {
+            v[i] = __uint_as_float(r[i]);
+          }
+        }
+        if constexpr (sizeof(TO) == 2) {
+          if (p.wide) {
+            store_chunk(out, v, strip, w.row0 + c, left, f_warp, p.N, lane);
+            continue;
+          }
+        }
+        if (f < p.N) {
+          TO* d = out + (int64_t)(w.row0 + c) * p.N + f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (i < left) d[(int64_t)i * p.N] = Elem<TO>::from_f(v[i]);
+        }
+      }
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster((tempty0 + 8 * acc) & kPeerMask);
+      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+    }
+  }
+
+  __syncwarp();
+  if (*abort_flag) settle();
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();          // nobody leaves while the peer may still touch its shared memory
+  if (warp == 1) {
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+// ---- weight gradient ---------------------------------------------------------------------------------
+constexpr int kWStages = 6;
+constexpr uint32_t kWHalfBytes = 128 * 128;              // 128 columns x 64 rows of one operand, two boxes
+constexpr uint32_t kWStageBytes = 2 * kWHalfBytes;
+constexpr uint32_t kWBoxBytes = 64 * 128;                // 64 columns x 64 rows
+
+struct WgradParams {
+  const int32_t* offsets;
+  __nv_bfloat16* out;
+  int32_t* fault;
+  int R, P, Q, E;
+};
+struct WgradItem {
+  int valid, e, p0, q0, row0, rows;
+};
+__device__ __forceinline__ WgradItem wgrad_item(const RowsOrder& o, const WgradParams& p, int item) {
+  WgradItem w;
+  const int qb = (p.Q + 255) / 256, per = (p.P + 255) / 256 * qb;
+  w.valid = item < p.E * per;
+  if (!w.valid) return w;
+  const int i = item / per, r = item - i * per;
+  w.e = o.order[i];
+  w.p0 = r / qb * 256;
+  w.q0 = r % qb * 256;
+  w.row0 = o.row0[w.e + 1];
+  w.rows = o.row0[w.e + 2] - w.row0;
+  return w;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kRThreads, 1)
+ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                       const __grid_constant__ WgradParams p) {
+  constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) |
+                              ((uint32_t)(256 >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  __shared__ __align__(8) uint64_t bars[3 * kWStages + 5];
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int abort_flag_s;
+  __shared__ RowsOrder ord;
+  __shared__ __align__(16) uint32_t strips[kREpiWarps][kRStripBytes / 4];
+  volatile int* abort_flag = &abort_flag_s;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[kWStages]), part0 = smem_u32(&bars[2 * kWStages]);
+  const uint32_t tfull0 = smem_u32(&bars[3 * kWStages]), tempty0 = smem_u32(&bars[3 * kWStages + 2]);
+  const uint32_t drain0 = smem_u32(&bars[3 * kWStages + 4]);
+  const uint32_t smem_base = smem_u32(smem);
+  const int cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
+  const int E = p.E;
+
+  if (warp == 0) load_spans(*reinterpret_cast<RaggedSpans*>(&ord), p.offsets, E, p.R, 256);
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&tmem_base_s)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  if (threadIdx.x == 64) {
+    abort_flag_s = 0;
+    mbar_init(drain0, 1);
+    for (int s = 0; s < kWStages; ++s) {
+      mbar_init(full0 + 8 * s, 2);                  // one arrival of either CTA
+      mbar_init(empty0 + 8 * s, 1);
+      mbar_init(part0 + 8 * s, 1);                  // this CTA's loads of a stage that the fixer takes
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull0 + 8 * a, 1);
+      mbar_init(tempty0 + 8 * a, 2 * kREpiWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += kRThreads) {
+    const int mine = ord.row0[e + 2] - ord.row0[e + 1];
+    int rk = 0;
+    for (int o = 0; o < E; ++o) {
+      const int other = ord.row0[o + 2] - ord.row0[o + 1];
+      rk += (other > mine) || (other == mine && o < e);
+    }
+    ord.order[rk] = (uint8_t)e;
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = tmem_base_s;
+
+  if (warp == 0) {
+    // ---- TMA producer: lanes 0, 1 the boxes of a, lanes 2, 3 those of b ----
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int item = cluster_id; ok; item += n_clusters) {
+      const WgradItem w = wgrad_item(ord, p, item);
+      if (!w.valid) break;
+      const int c0 = (lane < 2 ? w.p0 : w.q0) + 128 * (int)rank + 64 * (lane & 1);
+      for (int r = 0; r < w.rows; r += 64) {
+        ok = warp_all_wait(empty0 + 8 * stage, phase ^ 1, abort_flag, p.fault, 71);
+        if (!ok) break;
+        const uint32_t dst = smem_base + stage * kWStageBytes + lane * kWBoxBytes;
+        if (w.rows - r < 64 && (w.rows & 15) != 0) {
+          // a stage for the fixer: this CTA's boxes land on its own barrier, the fixer arrives
+          if (lane == 0) mbar_expect_tx(part0 + 8 * stage, kWStageBytes);
+          __syncwarp();
+          if (lane < 4) tma_load_2d(dst, lane < 2 ? &map_a : &map_b, part0 + 8 * stage, c0, w.row0 + r);
+        } else {
+          const uint32_t bar = (full0 + 8 * stage) & kPeerMask;
+          if (lane == 0) {
+            if (rank == 0) mbar_expect_tx(full0 + 8 * stage, 2u * kWStageBytes);
+            else mbar_arrive_cluster(bar);
+          }
+          __syncwarp();
+          if (lane < 4) tma2_load_2d(dst, lane < 2 ? &map_a : &map_b, bar, c0, w.row0 + r);
+        }
+        if (++stage == kWStages) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    // ---- MMA issuer (even CTA) ----
+    if (lane == 0 && rank == 0) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int item = cluster_id; ok; item += n_clusters) {
+        const WgradItem w = wgrad_item(ord, p, item);
+        if (!w.valid) break;
+        if (w.rows == 0) continue;
+        if (!(ok = mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag, p.fault, 72))) break;
+        tcgen05_fence_after();
+        const uint32_t d_tmem = tmem_base + 256 * acc;
+        for (int r = 0; r < w.rows; r += 64) {
+          if (!(ok = mbar_wait_cluster(full0 + 8 * stage, phase, abort_flag, p.fault, 73))) break;
+          tcgen05_fence_after();
+          const uint32_t sa = smem_base + stage * kWStageBytes, sb = sa + kWHalfBytes;
+          auto mma = [&](int ks) {
+            tcgen05_mma2_bf16(d_tmem, make_desc(sa + ks * (16 * 128), kWBoxBytes, 1024),
+                              make_desc(sb + ks * (16 * 128), kWBoxBytes, 1024), kIdesc, (r | ks) ? 1u : 0u);
+          };
+          const int left = w.rows - r;
+          if (left >= 64) {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) mma(ks);
+          } else {
+            for (int ks = 0; ks * 16 < left; ++ks) mma(ks);
+          }
+          tcgen05_commit2(empty0 + 8 * stage);
+          if (++stage == kWStages) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        tcgen05_commit2(tfull0 + 8 * acc);
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      }
+      if (*abort_flag) {
+        tcgen05_commit2(drain0);
+        mbar_drain(drain0, 0, globaltimer_ns() + 200000000ull);
+      }
+    }
+  } else if (warp == 2) {
+    // ---- fixer (both CTAs): zeros over the rows of others in an expert's last 16-row step ----
+    int stage = 0;
+    uint32_t seen = 0;                              // bit s: parity of the uses of part0[s] so far
+    for (int item = cluster_id;; item += n_clusters) {
+      const WgradItem w = wgrad_item(ord, p, item);
+      if (!w.valid) break;
+      if (w.rows == 0) continue;
+      const int n = (w.rows + 63) / 64;
+      const int last = (stage + n - 1) % kWStages;
+      stage = (stage + n) % kWStages;
+      if ((w.rows & 15) == 0) continue;
+      if (!warp_all_wait(part0 + 8 * last, (seen >> last) & 1u, abort_flag, p.fault, 74)) break;
+      seen ^= 1u << last;
+      const int valid = (w.rows - 1) % 64 + 1, end = (valid + 15) & ~15;
+      // a box's row is 128 bytes; four boxes; the swizzle moves 16-byte pieces within a row only
+      const int pieces = (end - valid) * 8;
+      uint8_t* base = smem + last * kWStageBytes + valid * 128;
+      for (int i = lane; i < 4 * pieces; i += 32)
+        *reinterpret_cast<uint4*>(base + (i / pieces) * kWBoxBytes + (i % pieces) * 16) = make_uint4(0, 0, 0, 0);
+      fence_async_proxy();                          // the tensor cores read through the async proxy
+      __syncwarp();
+      if (lane == 0) mbar_arrive_release_cluster((full0 + 8 * last) & kPeerMask);
+    }
+  } else if (warp >= 4) {
+    // ---- epilogue (both CTAs): warp -> 32 rows of the gradient, 64 columns ----
+    const int quarter = warp & 3, grp = (warp - 4) >> 2;
+    uint8_t* strip = reinterpret_cast<uint8_t*>(strips[warp - 4]);
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int item = cluster_id;; item += n_clusters) {
+      const WgradItem w = wgrad_item(ord, p, item);
+      if (!w.valid) break;
+      const bool empty = w.rows == 0;               // no rows: the gradient is zero
+      if (!empty) {
+        if (!warp_all_wait(tfull0 + 8 * acc, acc_phase, abort_flag, p.fault, 75)) break;
+        tcgen05_fence_after();
+      }
+      const int prow = w.p0 + 128 * (int)rank + 32 * quarter;     // of lane 0
+      const int qcol = w.q0 + 64 * grp;
+      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + 256 * acc + 64 * grp;
+      uint32_t o[4][8];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        uint32_t r[16];
+        if (!empty) {
+          tmem_ld16(taddr + 16 * s, r);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) r[i] = 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[s][i] = two_bf16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+      }
+      if (!empty) {
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster((tempty0 + 8 * acc) & kPeerMask);
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      }
+      // through the strip in four passes of eight rows (128 bytes each), 16-byte pieces swizzled by the
+      // row: a store instruction then writes whole 128-byte lines
+      __nv_bfloat16* out = p.out + ((int64_t)w.e * p.P + prow) * p.Q + qcol;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        __syncwarp();
+        if ((lane >> 3) == j) {
+          const int rr = lane & 7;
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+              *reinterpret_cast<uint4*>(strip + rr * 128 + (((2 * s + hf) ^ rr) << 4)) =
+                  make_uint4(o[s][4 * hf], o[s][4 * hf + 1], o[s][4 * hf + 2], o[s][4 * hf + 3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int rr = (lane >> 3) + 4 * k, piece = lane & 7;
+          const uint4 v = *reinterpret_cast<const uint4*>(strip + rr * 128 + ((piece ^ rr) << 4));
+          if (prow + 8 * j + rr < p.P && qcol + 8 * piece < p.Q)
+            *reinterpret_cast<uint4*>(out + (int64_t)(8 * j + rr) * p.Q + 8 * piece) = v;
+        }
+      }
+    }
+  }
+
+  __syncwarp();
+  if (*abort_flag) settle();
+  __syncwarp();
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+  }
+}
+
+// ---- host side ---------------------------------------------------------------------------------------
+// Pairs of CTAs that are resident at once with the kernel's largest shared memory
+template <typename Kern>
+static int resident_pairs(Kern kern, size_t smem, PerDeviceInt& cache, int* pairs) {
+  const int dev = current_device();
+  int n = (int)cache.get(dev);
+  if (n == 0) {
+    MOLE_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (sm_count() / 2));
+    cfg.blockDim = dim3(kRThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = sm_count() / 2;
+    }
+    cache.set(dev, n);
+  }
+  *pairs = n;
+  return MOLE_OK;
+}
+
+constexpr size_t kRBudget = 192 * 1024 + 1024;           // dynamic shared memory, next to the static 22 KB
+
+template <bool I8, bool KN, typename TO>
+static int launch_rows(const RowsMaps& maps, RowsParams p, int64_t max_items, cudaStream_t st) {
+  auto kern = ragged_rows_tc_kernel<I8, KN, TO>;
+  static PerDeviceInt cache;
+  int pairs = 0;
+  if (int rc = resident_pairs(kern, kRBudget, cache, &pairs)) return rc;
+  if (max_items < pairs) pairs = (int)max_items;
+  const size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
+  kern<<<2 * pairs, kRThreads, smem, st>>>(maps, p);
+  MOLE_LAUNCH_OK();
+  return MOLE_OK;
+}
+
+bool ragged_rows_tc_takes(int elem, const RaggedRows& a) {
+  const int unit = 16 / elem;                            // elements per 16 bytes
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w);
+  return a.K % unit == 0 && (!a.kn || a.N % unit == 0) && (bases & 15) == 0;
+}
+
+int ragged_rows_tc(int elem, int out_dtype, const RaggedRows& a, cudaStream_t st) {
+  RowsMaps maps;
+  const uint32_t kb = 128 / elem;
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t dims[2] = {(uint64_t)a.K, (uint64_t)a.R};
+    const uint32_t box[2] = {kb, (uint32_t)(64 >> i)};
+    if (int rc = encode_map(&maps.x[i], a.x, 2, dims, box, elem)) return rc;
+  }
+  const uint64_t dims[3] = {(uint64_t)(a.kn ? a.N : a.K), (uint64_t)(a.kn ? a.K : a.N), (uint64_t)a.E};
+  const uint32_t box_k[3] = {kb, 128, 1}, box_n[3] = {64, 64, 1};
+  if (int rc = encode_map(&maps.w, a.w, 3, dims, a.kn ? box_n : box_k, elem)) return rc;
+  RowsParams p{};
+  p.offsets = a.offsets; p.x_scale = a.x_scale; p.w_scale = a.w_scale; p.out = a.out;
+  p.fault = device_fault_word();
+  MOLE_REQUIRE(p.fault != nullptr, "fault word not allocated");
+  p.R = (int)a.R; p.N = a.N; p.E = a.E;
+  p.nkb = (int)((a.K + kb - 1) / kb);
+  const size_t osize = out_dtype == MOLE_F32 ? 4 : 2;
+  p.wide = a.N * osize % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+  // no panel has more than min(256, R) rows: few rows leave the shared memory to more stages
+  const int step = elem == 1 ? 32 : 16;
+  const int n_max = a.R >= 256 ? 256 : (int)((a.R + step - 1) / step * step);
+  p.stage_bytes = kRABytes + (uint32_t)(n_max / 2) * 128u;
+  p.stage_bytes = (p.stage_bytes + 1023) & ~1023u;
+  p.stages = (int)((kRBudget - 1024) / p.stage_bytes);
+  if (p.stages > kRMaxStages) p.stages = kRMaxStages;
+  const int64_t panels = a.R / 256 + (a.E < a.R ? a.E : a.R);       // every expert may end in a partial one
+  const int64_t items = panels * ((a.N + 255) / 256);
+  if (elem == 1) {
+    if (out_dtype == MOLE_F32) return launch_rows<true, false, float>(maps, p, items, st);
+    return launch_rows<true, false, __nv_bfloat16>(maps, p, items, st);
+  }
+  if (a.kn) return launch_rows<false, true, __nv_bfloat16>(maps, p, items, st);
+  return launch_rows<false, false, __nv_bfloat16>(maps, p, items, st);
+}
+
+bool ragged_wgrad_tc_takes(const RaggedWgrad& a) {
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(a.a) | reinterpret_cast<uintptr_t>(a.b) | reinterpret_cast<uintptr_t>(a.out);
+  return a.R > 0 && a.P % 8 == 0 && a.Q % 8 == 0 && (bases & 15) == 0;
+}
+
+int ragged_wgrad_tc(const RaggedWgrad& a, cudaStream_t st) {
+  CUtensorMap ma, mb;
+  const uint32_t box[2] = {64, 64};
+  const uint64_t da[2] = {(uint64_t)a.P, (uint64_t)a.R}, db[2] = {(uint64_t)a.Q, (uint64_t)a.R};
+  if (int rc = encode_map(&ma, a.a, 2, da, box, 2)) return rc;
+  if (int rc = encode_map(&mb, a.b, 2, db, box, 2)) return rc;
+  WgradParams p{};
+  p.offsets = a.offsets;
+  p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.fault = device_fault_word();
+  MOLE_REQUIRE(p.fault != nullptr, "fault word not allocated");
+  p.R = (int)a.R; p.P = a.P; p.Q = a.Q; p.E = a.E;
+  constexpr size_t smem = (size_t)kWStages * kWStageBytes + 1024;
+  static PerDeviceInt cache;
+  int pairs = 0;
+  if (int rc = resident_pairs(ragged_wgrad_tc_kernel, smem, cache, &pairs)) return rc;
+  const int64_t items = (int64_t)a.E * ((a.P + 255) / 256) * ((a.Q + 255) / 256);
+  MOLE_REQUIRE(items < (1ll << 31), "%d experts of %d x %d", a.E, a.P, a.Q);
+  if (items < pairs) pairs = (int)items;
+  ragged_wgrad_tc_kernel<<<2 * pairs, kRThreads, smem, st>>>(ma, mb, p);
+  MOLE_LAUNCH_OK();
+  return MOLE_OK;
+}
+
+}  // namespace mole
