@@ -22,6 +22,7 @@
 #include <type_traits>
 #include <unordered_map>
 
+#include "f32x2.cuh"
 #include "gemm.cuh"
 #include "tc_ptx.cuh"
 
@@ -235,30 +236,6 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // Pairs of values on the packed fp32 instructions (fma / mul / add .f32x2): the FC1 and dX2
 // epilogues are bound by instruction issue, and the pair forms do the same operations in the same
 // order as the scalar code in about half the instructions (results are bit-identical).
-__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t f2_dup(float a) { return f2_pack(a, a); }
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // gelu_parts on two values: the same operations in the same order
 struct GeluParts2 { uint64_t cdf, e; };
 __device__ __forceinline__ GeluParts2 gelu_parts2(uint64_t x) {
