@@ -19,7 +19,7 @@ CSRC = HERE / "csrc"
 OUT_DIR = HERE / "lib"
 LIB = OUT_DIR / "libmole_b200.so"
 SOURCES = ["route.cu", "dispatch.cu", "gate_mma.cu", "gemm_simt.cu", "gemm_tc.cu", "ffn.cu", "runtime.cu", "adam.cu",
-           "adam_multi.cu", "ragged.cu", "ragged_simt.cu", "ragged_tc.cu"]
+           "adam_multi.cu", "ragged.cu", "ragged_simt.cu", "ragged_tc.cu", "ragged_few.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

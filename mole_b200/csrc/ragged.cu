@@ -20,33 +20,63 @@ __device__ __forceinline__ int quantize_one(float x, float scale, float inv) {
   return (int)fminf(fmaxf(r, -127.f), 127.f);
 }
 
-template <typename T, int V>
+// One row per group of G threads (a warp or a block).  HELD: the row fits the group's registers (eight
+// 16-byte vectors a thread), is read once and waits there for its scale; otherwise it is read twice.
+// V = 1: rows that 16-byte loads cannot address.
+// Bound by HBM (3 bytes an element of bf16): 32768 x 2048 in 41 us, 4.9 TB/s.
+template <typename T, int V, int G, bool HELD>
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const T* __restrict__ x, int64_t R, int K, int8_t* __restrict__ q, float* __restrict__ scale) {
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= R) return;
-  const int lane = threadIdx.x & 31;
+  constexpr int kHeld = 8;
+  __shared__ uint32_t tops[8];
+  const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+  if (row >= R) return;                                      // a whole warp, or the whole block
+  const int t = threadIdx.x % G;
   const T* xr = x + row * K;
-  uint32_t top = 0;                                          // of the magnitudes' bits: NaN above infinity above all
-  for (int k = lane * V; k < K; k += 32 * V) {
-    float v[V];
+  auto load = [&](int k, float (&v)[V]) {
     if constexpr (V > 1) Vec16<T>::load(xr + k, v);
     else v[0] = Elem<T>::to_f(xr[k]);
+  };
+  uint4 held[kHeld];
+  uint32_t top = 0;                                          // of the magnitudes' bits: NaN above infinity above all
+  auto see = [&](const float (&v)[V]) {
 #pragma unroll
     for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+  };
+  if constexpr (HELD) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      const int k = (j * G + t) * V;
+      held[j] = k < K ? *reinterpret_cast<const uint4*>(xr + k) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      float v[V];
+      Vec16<T>::load(reinterpret_cast<const T*>(&held[j]), v);
+      see(v);
+    }
+  } else {
+    for (int k = t * V; k < K; k += G * V) {
+      float v[V];
+      load(k, v);
+      see(v);
+    }
   }
   top = __reduce_max_sync(0xffffffffu, top);
+  if (G > 32) {
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < G / 32; ++w) top = max(top, tops[w]);
+  }
   const float s = __fdiv_rn(__uint_as_float(top), 127.f);
-  if (lane == 0) scale[row] = s;
+  if (t == 0) scale[row] = s;
   const bool zero = !(s > 0.f && s < __int_as_float(0x7f800000));    // all zero, or not finite: the scale says it
   // rows of tiny values: both sides times 2^100, so that neither 1 / scale overflows nor the
-  // difference above leaves the range of fp32
+  // difference in quantize_one leaves the range of fp32
   const float up = s < 0x1p-100f ? 0x1p100f : 1.f;
   const float su = s * up, inv = zero ? 0.f : __fdiv_rn(1.f, su);
-  for (int k = lane * V; k < K; k += 32 * V) {
-    float v[V];
-    if constexpr (V > 1) Vec16<T>::load(xr + k, v);
-    else v[0] = Elem<T>::to_f(xr[k]);
+  auto store = [&](int k, const float (&v)[V]) {
     uint32_t w[(V + 3) / 4] = {};
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -57,18 +87,38 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t R, int K, int8_t* __restri
     if constexpr (V == 8) *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
     else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(d) = w[0];
     else *d = (int8_t)w[0];
+  };
+  if constexpr (HELD) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      const int k = (j * G + t) * V;
+      float v[V];
+      Vec16<T>::load(reinterpret_cast<const T*>(&held[j]), v);
+      if (k < K) store(k, v);
+    }
+  } else {
+    for (int k = t * V; k < K; k += G * V) {
+      float v[V];
+      load(k, v);
+      store(k, v);
+    }
   }
 }
 
 template <typename T>
 static int launch_quantize(const void* x, int64_t R, int K, void* q, float* scale, cudaStream_t st) {
   constexpr int V = Vec16<T>::N;
-  const unsigned grid = (unsigned)((R + 7) / 8);
   const bool wide = K % V == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & (V - 1)) == 0;
-  if (wide)
-    quantize_rows_kernel<T, V><<<grid, 256, 0, st>>>(static_cast<const T*>(x), R, K, static_cast<int8_t*>(q), scale);
-  else
-    quantize_rows_kernel<T, 1><<<grid, 256, 0, st>>>(static_cast<const T*>(x), R, K, static_cast<int8_t*>(q), scale);
+  const T* xp = static_cast<const T*>(x);
+  int8_t* qp = static_cast<int8_t*>(q);
+  // a warp a row while rows are short and fill the SMs, else a block a row
+  const bool block = K > 32 * V * 8 || R < (int64_t)sm_count() * 16;
+  const unsigned grid = (unsigned)(block ? R : (R + 7) / 8);
+  if (wide && block && K <= 256 * V * 8) quantize_rows_kernel<T, V, 256, true><<<grid, 256, 0, st>>>(xp, R, K, qp, scale);
+  else if (wide && block) quantize_rows_kernel<T, V, 256, false><<<grid, 256, 0, st>>>(xp, R, K, qp, scale);
+  else if (wide) quantize_rows_kernel<T, V, 32, true><<<grid, 256, 0, st>>>(xp, R, K, qp, scale);
+  else if (block) quantize_rows_kernel<T, 1, 256, false><<<grid, 256, 0, st>>>(xp, R, K, qp, scale);
+  else quantize_rows_kernel<T, 1, 32, false><<<grid, 256, 0, st>>>(xp, R, K, qp, scale);
   MOLE_LAUNCH_OK();
   return MOLE_OK;
 }
@@ -97,6 +147,7 @@ extern "C" int mole_grouped_mm(const void* x, const void* w, const int32_t* offs
   RaggedRows a{};
   a.x = x; a.w = w; a.offsets = offsets; a.out = out;
   a.R = R; a.N = N; a.K = K; a.E = E; a.kn = w_kn != 0;
+  if (ragged_rows_few_takes(a)) return ragged_rows_few(dtype, a, static_cast<cudaStream_t>(stream));
   if (dtype == MOLE_BF16 && ragged_rows_tc_takes(2, a)) return ragged_rows_tc(2, dtype, a, static_cast<cudaStream_t>(stream));
   return ragged_rows_simt(dtype, a, static_cast<cudaStream_t>(stream));
 }
@@ -119,7 +170,7 @@ extern "C" int mole_grouped_mm_wgrad(const void* a, const void* b, const int32_t
 
 extern "C" int mole_quantize_rows(const void* x, int64_t R, int32_t K, int32_t dtype, void* q,
                                   float* scale, void* stream) {
-  MOLE_REQUIRE(R >= 0 && R < (1ll << 33), "rows=%lld", (long long)R);
+  MOLE_REQUIRE(R >= 0 && R < (1ll << 31), "rows=%lld", (long long)R);
   MOLE_REQUIRE(K >= 1 && K <= (1 << 21), "K=%d", K);
   MOLE_REQUIRE(dtype == MOLE_F32 || dtype == MOLE_BF16, "dtype %d", dtype);
   if (R == 0) return MOLE_OK;
@@ -144,6 +195,7 @@ extern "C" int mole_grouped_mm_i8(const void* q, const float* q_scale, const voi
   RaggedRows a{};
   a.x = q; a.w = w; a.offsets = offsets; a.x_scale = q_scale; a.w_scale = w_scale; a.out = out;
   a.R = R; a.N = N; a.K = K; a.E = E;
+  if (ragged_rows_few_takes(a)) return ragged_rows_few_i8(out_dtype, a, static_cast<cudaStream_t>(stream));
   if (ragged_rows_tc_takes(1, a)) return ragged_rows_tc(1, out_dtype, a, static_cast<cudaStream_t>(stream));
   return ragged_rows_simt_i8(out_dtype, a, static_cast<cudaStream_t>(stream));
 }

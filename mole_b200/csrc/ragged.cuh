@@ -31,6 +31,10 @@ struct RaggedWgrad {        // out[e, p, q] = sum over the rows r of e of a[r, p
 int ragged_rows_simt(int dtype, const RaggedRows& a, cudaStream_t st);
 int ragged_rows_simt_i8(int out_dtype, const RaggedRows& a, cudaStream_t st);
 int ragged_wgrad_simt(int dtype, const RaggedWgrad& a, cudaStream_t st);
+// up to 16 rows
+bool ragged_rows_few_takes(const RaggedRows& a);
+int ragged_rows_few(int dtype, const RaggedRows& a, cudaStream_t st);
+int ragged_rows_few_i8(int out_dtype, const RaggedRows& a, cudaStream_t st);
 // tensor cores, where rows and weights can be addressed by TMA (elem 2 = bf16, 1 = 8-bit integers)
 bool ragged_rows_tc_takes(int elem, const RaggedRows& a);
 int ragged_rows_tc(int elem, int out_dtype, const RaggedRows& a, cudaStream_t st);

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import itertools
 import math
 from dataclasses import dataclass
 from typing import Optional, Sequence
@@ -442,8 +443,8 @@ def adam_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     ``v = (code * scale) ** 2``; zeros are a fresh state).  8-bit moments are rounded at random by
     bits that ``seed``, ``t``, the place in the list and the element determine: the same call gives
     the same bits."""
-    n = len(params)
     lists = [params, grads, exp_avgs, exp_avg_sqs]
+    n = len(params)
     if n == 0:
         return
     bits = 8 if exp_avgs[0].dtype == torch.float8_e4m3fn else 32
@@ -456,32 +457,35 @@ def adam_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     if any(len(x) != n for x in lists):
         raise ValueError("one gradient, two moments (and their scales) per parameter")
     dt = _dt(params[0])
-    dtype, device = params[0].dtype, params[0].device
+    # The checks run list by list over C-level methods: a step over hundreds of small tensors takes no
+    # longer on the GPU than on the host.
+    dtype, index = params[0].dtype, params[0].get_device()
+    if not params[0].is_cuda:
+        raise RuntimeError("mole_b200 kernels take CUDA tensors only (there is no CPU path)")
+    if any(set(map(torch.Tensor.get_device, xs)) != {index} for xs in lists):
+        raise ValueError("the tensors are on different devices")
     mdtype = torch.float8_e4m3fn if bits == 8 else torch.float32
-    table = (AdamTensor * n)()
-    seen = set()
-    for i, ts in enumerate(zip(*lists)):
-        p, g, m, v = ts[:4]
-        size = p.numel()
-        if p.dtype != dtype or g.dtype != dtype:
-            raise TypeError(f"tensor {i}: parameter and gradient must both be {dtype}")
-        if m.dtype != mdtype or v.dtype != mdtype:
-            raise TypeError(f"tensor {i}: both moments must be {mdtype}")
-        if g.numel() != size or m.numel() != size or v.numel() != size:
-            raise ValueError(f"tensor {i}: parameter, gradient and moments differ in size")
-        for x in ts:
-            if x.device != device:
-                raise ValueError(f"tensor {i}: tensors are on different devices: {device} and {x.device}")
-        e = table[i]
-        e.p, e.g, e.m, e.v, e.n = _ptr(p), _ptr(g), _ptr(m), _ptr(v), size
-        if bits == 8:
-            for x in ts[4:]:
-                if x.dtype != torch.float32 or x.numel() != adam_scales(size):
-                    raise ValueError(f"tensor {i}: scales must be float32 [{adam_scales(size)}]")
-            e.m_scale, e.v_scale = _ptr(ts[4]), _ptr(ts[5])
-        if size and (e.p in seen):
-            raise ValueError(f"tensor {i}: the same parameter twice in one call")
-        seen.add(e.p)
+    for xs, want, what in zip(lists, (dtype, dtype, mdtype, mdtype, torch.float32, torch.float32),
+                              ("parameters", "gradients", "moments", "moments", "scales", "scales")):
+        if {x.dtype for x in xs} != {want}:
+            raise TypeError(f"the {what} must all be {want}")
+        if not all(map(torch.Tensor.is_contiguous, xs)):
+            raise RuntimeError("mole_b200 kernels take contiguous tensors")
+    sizes = list(map(torch.Tensor.numel, params))
+    if any(list(map(torch.Tensor.numel, xs)) != sizes for xs in lists[1:4]):
+        raise ValueError("parameters, gradients and moments differ in size")
+    if bits == 8:
+        blocks = [-(-k // ADAM_BLOCK) for k in sizes]
+        if any(list(map(torch.Tensor.numel, xs)) != blocks for xs in lists[4:]):
+            raise ValueError(f"scales must be float32, one per {ADAM_BLOCK} elements")
+    columns = [list(map(torch.Tensor.data_ptr, xs)) for xs in lists]
+    held = [q for q in columns[0] if q]
+    if len(set(held)) != len(held):
+        raise ValueError("the same parameter twice in one call")
+    if bits == 32:
+        columns += [[0] * n] * 2
+    words = (C.c_uint64 * (7 * n))(*itertools.chain.from_iterable(zip(*columns, sizes)))
+    table = C.cast(words, C.POINTER(AdamTensor))
     with _on_device_of(params[0]):
         check(lib.mole_adam_multi(table, n, dt, bits, betas[0], betas[1], int(t), float(lr),
                                   float(weight_decay), float(eps), int(bool(adamw)),

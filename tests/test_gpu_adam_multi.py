@@ -312,9 +312,9 @@ def test_refusals():
         go(args(ms=[s["ms"][0], s["ms"][0][:0]]))
     with pytest.raises(ValueError, match="differ in size"):
         go(args(g=[s["g"][0], s["g"][0]]))
-    with pytest.raises(TypeError, match="both be"):
+    with pytest.raises(TypeError, match="gradients must all be"):
         go(args(g=[s["g"][0], s["g"][1].bfloat16()]))
-    with pytest.raises(TypeError, match="moments"):
+    with pytest.raises(TypeError, match="moments must all be"):
         go(args(v=[s["v"][0], s["v"][1].float()]))
     with pytest.raises(ValueError, match="one gradient"):
         go(args(g=s["g"][:1]))
