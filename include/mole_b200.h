@@ -307,19 +307,28 @@ int mole_ffn_bwd_peer(const mole_ffn_desc* desc, const int32_t* counts,
  * the device, as mole_gate_route_fwd writes them; E <= 256; an expert may have no rows).  Rows before
  * offsets[0] and from offsets[E] on belong to nobody: products write zeros there.  The offsets are
  * clamped on the device to a rising sequence in [0, R].  Any width and element-aligned pointers are
- * taken; widths that are multiples of 8 (16 for 8-bit integers) with 16-byte aligned pointers run on
- * the tensor cores for bf16 and 8-bit integers.  All sums are held in 32 bits and rounded once.
+ * taken; operands of bf16 and 8-bit integers whose rows do not start on 16 bytes are first copied
+ * into the workspace, whose size mole_grouped_mm_workspace_bytes gives (0, and null will do, where
+ * all rows do, for fp32, and for up to 16 rows).  All sums are held in 32 bits and rounded once.
  * The reference computes the same products inside bffn_fwd / bffn_bwd over capacity-padded rows
  * (MOLE/cpp/core.cpp:350-353, 388-412).
  * ---------------------------------------------------------------------------------- */
 /* out[r, n] = sum_k x[r, k] w_e(n, k) for r of expert e: w is [E, N, K] (w_kn = 0) or [E, K, N]
  * (w_kn = 1).  The gradient of x is the same call on dout with the other w_kn. */
 int mole_grouped_mm(const void* x, const void* w, const int32_t* offsets, int64_t R, int32_t N,
-                    int32_t K, int32_t E, int32_t w_kn, int32_t dtype, void* out, void* stream);
+                    int32_t K, int32_t E, int32_t w_kn, int32_t dtype, void* out, void* workspace,
+                    int64_t workspace_bytes, void* stream);
+/* elem_bytes 4, 2 or 1: fp32, bf16, or the operands of mole_grouped_mm_i8 (w_kn = 0).  Of x and w only the
+ * alignment of the addresses counts. */
+int mole_grouped_mm_workspace_bytes(const void* x, const void* w, int64_t R, int32_t N, int32_t K,
+                                    int32_t E, int32_t w_kn, int32_t elem_bytes, int64_t* bytes);
 /* out[e, p, q] = sum over the rows r of e of a[r, p] b[r, q]: the weight gradient, zeros for an expert
  * without rows */
 int mole_grouped_mm_wgrad(const void* a, const void* b, const int32_t* offsets, int64_t R, int32_t P,
-                          int32_t Q, int32_t E, int32_t dtype, void* out, void* stream);
+                          int32_t Q, int32_t E, int32_t dtype, void* out, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+int mole_grouped_mm_wgrad_workspace_bytes(const void* a, const void* b, int64_t R, int32_t P, int32_t Q,
+                                          int32_t E, int32_t dtype, int64_t* bytes);
 /* q[r, k] = the integer in [-127, 127] nearest to x[r, k] / scale[r] (ties to even, decided exactly),
  * scale[r] = max_k |x[r, k]| / 127 rounded to fp32.  A row with a value that is not finite gets a
  * scale that is not finite and zeros: its products come out NaN. */
@@ -329,7 +338,8 @@ int mole_quantize_rows(const void* x, int64_t R, int32_t K, int32_t dtype, void*
  * the sum exact in 32 bits, out in out_dtype.  offsets may be null for E = 1 (every row belongs to it). */
 int mole_grouped_mm_i8(const void* q, const float* q_scale, const void* w, const float* w_scale,
                        const int32_t* offsets, int64_t R, int32_t N, int32_t K, int32_t E,
-                       int32_t out_dtype, void* out, void* stream);
+                       int32_t out_dtype, void* out, void* workspace, int64_t workspace_bytes,
+                       void* stream);
 
 /* ------------------------------------------------------------------------------------
  * streams.  Replaces the 16-stream manager (MOLE/cpp/stream.cpp:38-144) and its wait

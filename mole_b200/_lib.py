@@ -74,10 +74,12 @@ SIGNATURES = {
                                        _p, _p, _p, _i32, _p, _p, _i64, _p]),
     "mole_ffn_bwd": (C.c_int, [C.POINTER(FfnDesc), _p, _pi32, _pi32, _p, _p, _p, _p, _p, _p,
                                _p, _p, _p, _p, _p, _p, _p, _i64, _p]),
-    "mole_grouped_mm": (C.c_int, [_p, _p, _p, _i64, _i32, _i32, _i32, _i32, _i32, _p, _p]),
-    "mole_grouped_mm_wgrad": (C.c_int, [_p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p]),
+    "mole_grouped_mm": (C.c_int, [_p, _p, _p, _i64, _i32, _i32, _i32, _i32, _i32, _p, _p, _i64, _p]),
+    "mole_grouped_mm_workspace_bytes": (C.c_int, [_p, _p, _i64, _i32, _i32, _i32, _i32, _i32, _pi64]),
+    "mole_grouped_mm_wgrad": (C.c_int, [_p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _i64, _p]),
+    "mole_grouped_mm_wgrad_workspace_bytes": (C.c_int, [_p, _p, _i64, _i32, _i32, _i32, _i32, _pi64]),
     "mole_quantize_rows": (C.c_int, [_p, _i64, _i32, _i32, _p, _p, _p]),
-    "mole_grouped_mm_i8": (C.c_int, [_p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p]),
+    "mole_grouped_mm_i8": (C.c_int, [_p, _p, _p, _p, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _i64, _p]),
     "mole_ctx_create": (C.c_int, [_i32, _i32, C.POINTER(_p)]),
     "mole_ctx_destroy": (C.c_int, [_p]),
     "mole_ctx_stream": (C.c_int, [_p, _i32, C.POINTER(_p)]),

@@ -1216,16 +1216,16 @@ static int make_map(CUtensorMap* m, const void* base, int rank, const uint64_t* 
 }
 
 int encode_map(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint32_t* box,
-               int elem) {
+               int elem, uint64_t row_bytes) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(MOLE_ERR_CUDA, "cuTensorMapEncodeTiled entry point not found");
   cuuint64_t gdim[3], gstride[2];
   cuuint32_t bdim[3], estr[3] = {1, 1, 1};
-  uint64_t stride = (uint64_t)elem;
+  uint64_t stride = row_bytes ? row_bytes : dims[0] * (uint64_t)elem;      // of the second dimension
   for (int i = 0; i < rank; ++i) {
     gdim[i] = dims[i];
     bdim[i] = box[i];
-    stride *= dims[i];
+    if (i > 0) stride *= dims[i];
     if (i < rank - 1) gstride[i] = stride;
   }
   MOLE_REQUIRE((reinterpret_cast<uintptr_t>(base) & 15) == 0, "tensor base %p not 16-byte aligned", base);

@@ -1,5 +1,7 @@
 // C entries of the products over rows packed by expert, and the quantisation of rows to 8-bit
 // integers that the integer product takes.
+#include <cstring>
+
 #include "ragged.cuh"
 
 namespace mole {
@@ -123,13 +125,74 @@ static int launch_quantize(const void* x, int64_t R, int K, void* q, float* scal
   return MOLE_OK;
 }
 
+// ---- operands that the tensor cores cannot address ------------------------------------------------
+// TMA wants rows that start on 16 bytes.  Operands of other widths or at other addresses are copied to
+// rows that do, in the caller's workspace; the copy costs a pass of HBM over the operand (weights:
+// only those of experts that have rows), the products on the CUDA cores an order of magnitude.
+// A thread stores 16 bytes; matrix m of `rows` rows belongs to expert m, one matrix belongs to all.
+template <typename T>
+__global__ void __launch_bounds__(256)
+align_rows_kernel(const T* __restrict__ src, int64_t rows, int cols, int ld, T* __restrict__ dst,
+                  const int32_t* __restrict__ offsets) {
+  constexpr int V = 16 / sizeof(T);
+  if (offsets != nullptr && offsets[blockIdx.y + 1] <= offsets[blockIdx.y]) return;
+  const int per_row = ld / V;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * per_row) return;
+  const int64_t r = i / per_row;
+  const int c = (int)(i - r * per_row) * V;
+  const T* s = src + ((int64_t)blockIdx.y * rows + r) * cols + c;
+  T v[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = c + j < cols ? s[j] : T(0);
+  uint4 o;
+  memcpy(&o, v, 16);
+  *reinterpret_cast<uint4*>(dst + ((int64_t)blockIdx.y * rows + r) * ld + c) = o;
+}
+
+static bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+struct Aligner {            // deals out the workspace, or only counts
+  uint8_t* at;
+  int64_t left, used;
+  bool count_only;
+};
+// *p: the operand, [matrices, rows, cols] elements of `elem` bytes; on return it and *ld can be addressed
+static int align_operand(Aligner& ws, const void** p, int64_t matrices, int64_t rows, int cols, int elem, int* ld,
+                         const int32_t* offsets, cudaStream_t st) {
+  const int unit = 16 / elem;
+  *ld = cols;
+  if (cols % unit == 0 && aligned_to(*p, 16)) return MOLE_OK;
+  *ld = (cols + unit - 1) / unit * unit;
+  const int64_t bytes = (matrices * rows * *ld * elem + 255) / 256 * 256;
+  ws.used += bytes;
+  if (ws.count_only) return MOLE_OK;
+  MOLE_REQUIRE(ws.at != nullptr && ws.used <= ws.left && aligned_to(ws.at, 16),
+               "workspace of %lld bytes, %lld needed (mole_grouped_mm_workspace_bytes)", (long long)ws.left, (long long)ws.used);
+  void* dst = ws.at + ws.used - bytes;
+  const dim3 grid((unsigned)((rows * (*ld / unit) + 255) / 256), (unsigned)matrices);
+  if (elem == 1)
+    align_rows_kernel<int8_t><<<grid, 256, 0, st>>>(static_cast<const int8_t*>(*p), rows, cols, *ld,
+                                                    static_cast<int8_t*>(dst), offsets);
+  else
+    align_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(*p), rows, cols, *ld,
+                                                      static_cast<uint16_t*>(dst), offsets);
+  MOLE_LAUNCH_OK();
+  *p = dst;
+  return MOLE_OK;
+}
+static int align_rows(RaggedRows& a, int elem, Aligner ws, int64_t* used, cudaStream_t st) {
+  if (int rc = align_operand(ws, &a.x, 1, a.R, a.K, elem, &a.ldx, nullptr, st)) return rc;
+  if (int rc = align_operand(ws, &a.w, a.E, a.kn ? a.K : a.N, a.kn ? a.N : a.K, elem, &a.ldw, a.offsets, st)) return rc;
+  if (used) *used = ws.used;
+  return MOLE_OK;
+}
+
 static int check_sizes(int64_t R, int a, int b, int E) {
   MOLE_REQUIRE(R >= 0 && R < (1ll << 31) - 65536, "rows=%lld", (long long)R);
   MOLE_REQUIRE(a >= 1 && b >= 1 && a <= (1 << 21) && b <= (1 << 21), "widths %d, %d", a, b);
   MOLE_REQUIRE(E >= 1 && E <= kMaxRaggedExperts, "E=%d (1..%d)", E, kMaxRaggedExperts);
   return MOLE_OK;
 }
-static bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 }  // namespace mole
 
@@ -137,7 +200,7 @@ using namespace mole;
 
 extern "C" int mole_grouped_mm(const void* x, const void* w, const int32_t* offsets, int64_t R,
                                int32_t N, int32_t K, int32_t E, int32_t w_kn, int32_t dtype,
-                               void* out, void* stream) {
+                               void* out, void* workspace, int64_t workspace_bytes, void* stream) {
   if (int rc = check_sizes(R, N, K, E)) return rc;
   MOLE_REQUIRE(dtype == MOLE_F32 || dtype == MOLE_BF16, "dtype %d", dtype);
   if (R == 0) return MOLE_OK;
@@ -147,14 +210,28 @@ extern "C" int mole_grouped_mm(const void* x, const void* w, const int32_t* offs
   RaggedRows a{};
   a.x = x; a.w = w; a.offsets = offsets; a.out = out;
   a.R = R; a.N = N; a.K = K; a.E = E; a.kn = w_kn != 0;
-  if (ragged_rows_few_takes(a)) return ragged_rows_few(dtype, a, static_cast<cudaStream_t>(stream));
-  if (dtype == MOLE_BF16 && ragged_rows_tc_takes(2, a)) return ragged_rows_tc(2, dtype, a, static_cast<cudaStream_t>(stream));
-  return ragged_rows_simt(dtype, a, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (ragged_rows_few_takes(a)) return ragged_rows_few(dtype, a, st);
+  if (dtype == MOLE_F32) return ragged_rows_simt(a, st);
+  if (int rc = align_rows(a, 2, Aligner{static_cast<uint8_t*>(workspace), workspace_bytes, 0, false}, nullptr, st)) return rc;
+  return ragged_rows_tc(2, dtype, a, st);
+}
+
+extern "C" int mole_grouped_mm_workspace_bytes(const void* x, const void* w, int64_t R, int32_t N, int32_t K, int32_t E,
+                                               int32_t w_kn, int32_t elem_bytes, int64_t* bytes) {
+  if (int rc = check_sizes(R, N, K, E)) return rc;
+  MOLE_REQUIRE(bytes != nullptr && (elem_bytes == 1 || elem_bytes == 2 || elem_bytes == 4), "bad argument");
+  RaggedRows a{};
+  a.x = x; a.w = w;
+  a.R = R; a.N = N; a.K = K; a.E = E; a.kn = w_kn != 0;
+  *bytes = 0;
+  if (elem_bytes == 4 || ragged_rows_few_takes(a)) return MOLE_OK;
+  return align_rows(a, elem_bytes, Aligner{nullptr, 0, 0, true}, bytes, nullptr);
 }
 
 extern "C" int mole_grouped_mm_wgrad(const void* a, const void* b, const int32_t* offsets, int64_t R,
                                      int32_t P, int32_t Q, int32_t E, int32_t dtype, void* out,
-                                     void* stream) {
+                                     void* workspace, int64_t workspace_bytes, void* stream) {
   if (int rc = check_sizes(R, P, Q, E)) return rc;
   MOLE_REQUIRE(dtype == MOLE_F32 || dtype == MOLE_BF16, "dtype %d", dtype);
   MOLE_REQUIRE((a && b) || R == 0, "null pointer argument");
@@ -164,8 +241,30 @@ extern "C" int mole_grouped_mm_wgrad(const void* a, const void* b, const int32_t
   RaggedWgrad g{};
   g.a = a; g.b = b; g.offsets = offsets; g.out = out;
   g.R = R; g.P = P; g.Q = Q; g.E = E;
-  if (dtype == MOLE_BF16 && ragged_wgrad_tc_takes(g)) return ragged_wgrad_tc(g, static_cast<cudaStream_t>(stream));
-  return ragged_wgrad_simt(dtype, g, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == MOLE_F32) return ragged_wgrad_simt(g, st);
+  if (R == 0) {
+    MOLE_CUDA_OK(cudaMemsetAsync(out, 0, (size_t)E * P * Q * size, st));
+    return MOLE_OK;
+  }
+  Aligner ws{static_cast<uint8_t*>(workspace), workspace_bytes, 0, false};
+  if (int rc = align_operand(ws, &g.a, 1, R, P, 2, &g.lda, nullptr, st)) return rc;
+  if (int rc = align_operand(ws, &g.b, 1, R, Q, 2, &g.ldb, nullptr, st)) return rc;
+  return ragged_wgrad_tc(g, st);
+}
+
+extern "C" int mole_grouped_mm_wgrad_workspace_bytes(const void* a, const void* b, int64_t R, int32_t P, int32_t Q,
+                                                     int32_t E, int32_t dtype, int64_t* bytes) {
+  if (int rc = check_sizes(R, P, Q, E)) return rc;
+  MOLE_REQUIRE(bytes != nullptr && (dtype == MOLE_F32 || dtype == MOLE_BF16), "bad argument");
+  *bytes = 0;
+  if (dtype == MOLE_F32 || R == 0) return MOLE_OK;
+  Aligner ws{nullptr, 0, 0, true};
+  int ld = 0;
+  if (int rc = align_operand(ws, &a, 1, R, P, 2, &ld, nullptr, nullptr)) return rc;
+  if (int rc = align_operand(ws, &b, 1, R, Q, 2, &ld, nullptr, nullptr)) return rc;
+  *bytes = ws.used;
+  return MOLE_OK;
 }
 
 extern "C" int mole_quantize_rows(const void* x, int64_t R, int32_t K, int32_t dtype, void* q,
@@ -183,7 +282,8 @@ extern "C" int mole_quantize_rows(const void* x, int64_t R, int32_t K, int32_t d
 
 extern "C" int mole_grouped_mm_i8(const void* q, const float* q_scale, const void* w, const float* w_scale,
                                   const int32_t* offsets, int64_t R, int32_t N, int32_t K, int32_t E,
-                                  int32_t out_dtype, void* out, void* stream) {
+                                  int32_t out_dtype, void* out, void* workspace, int64_t workspace_bytes,
+                                  void* stream) {
   if (int rc = check_sizes(R, N, K, E)) return rc;
   MOLE_REQUIRE(out_dtype == MOLE_F32 || out_dtype == MOLE_BF16, "dtype %d", out_dtype);
   // |q w| <= 2^14: more terms could leave 32 bits
@@ -195,7 +295,8 @@ extern "C" int mole_grouped_mm_i8(const void* q, const float* q_scale, const voi
   RaggedRows a{};
   a.x = q; a.w = w; a.offsets = offsets; a.x_scale = q_scale; a.w_scale = w_scale; a.out = out;
   a.R = R; a.N = N; a.K = K; a.E = E;
-  if (ragged_rows_few_takes(a)) return ragged_rows_few_i8(out_dtype, a, static_cast<cudaStream_t>(stream));
-  if (ragged_rows_tc_takes(1, a)) return ragged_rows_tc(1, out_dtype, a, static_cast<cudaStream_t>(stream));
-  return ragged_rows_simt_i8(out_dtype, a, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (ragged_rows_few_takes(a)) return ragged_rows_few_i8(out_dtype, a, st);
+  if (int rc = align_rows(a, 1, Aligner{static_cast<uint8_t*>(workspace), workspace_bytes, 0, false}, nullptr, st)) return rc;
+  return ragged_rows_tc(1, out_dtype, a, st);
 }

@@ -18,6 +18,7 @@ struct RaggedRows {         // out[r, n] = sum_k x[r, k] w_e(n, k)
   void* out;                // [R, N]
   int64_t R;
   int N, K, E, kn;
+  int ldx, ldw;             // elements between rows of x, and of w's inner matrices
 };
 struct RaggedWgrad {        // out[e, p, q] = sum over the rows r of e of a[r, p] b[r, q]
   const void* a;            // [R, P]
@@ -26,19 +27,17 @@ struct RaggedWgrad {        // out[e, p, q] = sum over the rows r of e of a[r, p
   void* out;                // [E, P, Q]
   int64_t R;
   int P, Q, E;
+  int lda, ldb;
 };
 
-int ragged_rows_simt(int dtype, const RaggedRows& a, cudaStream_t st);
-int ragged_rows_simt_i8(int out_dtype, const RaggedRows& a, cudaStream_t st);
-int ragged_wgrad_simt(int dtype, const RaggedWgrad& a, cudaStream_t st);
-// up to 16 rows
+int ragged_rows_simt(const RaggedRows& a, cudaStream_t st);          // fp32
+int ragged_wgrad_simt(const RaggedWgrad& a, cudaStream_t st);
+// up to 16 rows, every type (ldx = K, ldw dense)
 bool ragged_rows_few_takes(const RaggedRows& a);
 int ragged_rows_few(int dtype, const RaggedRows& a, cudaStream_t st);
 int ragged_rows_few_i8(int out_dtype, const RaggedRows& a, cudaStream_t st);
-// tensor cores, where rows and weights can be addressed by TMA (elem 2 = bf16, 1 = 8-bit integers)
-bool ragged_rows_tc_takes(int elem, const RaggedRows& a);
+// tensor cores; elem 2 = bf16, 1 = 8-bit integers.  Rows of every operand start on 16 bytes (base and ld).
 int ragged_rows_tc(int elem, int out_dtype, const RaggedRows& a, cudaStream_t st);
-bool ragged_wgrad_tc_takes(const RaggedWgrad& a);
 int ragged_wgrad_tc(const RaggedWgrad& a, cudaStream_t st);
 
 constexpr int kMaxRaggedExperts = 256;

@@ -390,6 +390,7 @@ struct WgradParams {
   __nv_bfloat16* out;
   int32_t* fault;
   int R, P, Q, E;
+  int wide;             // rows of out are multiples of 16 bytes, its base too
 };
 struct WgradItem {
   int valid, e, p0, q0, row0, rows;
@@ -618,8 +619,17 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
         for (int k = 0; k < 2; ++k) {
           const int rr = (lane >> 3) + 4 * k, piece = lane & 7;
           const uint4 v = *reinterpret_cast<const uint4*>(strip + rr * 128 + ((piece ^ rr) << 4));
-          if (prow + 8 * j + rr < p.P && qcol + 8 * piece < p.Q)
-            *reinterpret_cast<uint4*>(out + (int64_t)(8 * j + rr) * p.Q + 8 * piece) = v;
+          if (prow + 8 * j + rr >= p.P) continue;
+          __nv_bfloat16* d = out + (int64_t)(8 * j + rr) * p.Q + 8 * piece;
+          const int left = p.Q - qcol - 8 * piece;
+          if (p.wide) {
+            if (left > 0) *reinterpret_cast<uint4*>(d) = v;
+          } else {
+            const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (i < left) d[i] = b[i];
+          }
         }
       }
     }
@@ -679,23 +689,17 @@ static int launch_rows(const RowsMaps& maps, RowsParams p, int64_t max_items, cu
   return MOLE_OK;
 }
 
-bool ragged_rows_tc_takes(int elem, const RaggedRows& a) {
-  const int unit = 16 / elem;                            // elements per 16 bytes
-  const uintptr_t bases = reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w);
-  return a.K % unit == 0 && (!a.kn || a.N % unit == 0) && (bases & 15) == 0;
-}
-
 int ragged_rows_tc(int elem, int out_dtype, const RaggedRows& a, cudaStream_t st) {
   RowsMaps maps;
   const uint32_t kb = 128 / elem;
   for (int i = 0; i < 4; ++i) {
     const uint64_t dims[2] = {(uint64_t)a.K, (uint64_t)a.R};
     const uint32_t box[2] = {kb, (uint32_t)(64 >> i)};
-    if (int rc = encode_map(&maps.x[i], a.x, 2, dims, box, elem)) return rc;
+    if (int rc = encode_map(&maps.x[i], a.x, 2, dims, box, elem, (uint64_t)a.ldx * elem)) return rc;
   }
   const uint64_t dims[3] = {(uint64_t)(a.kn ? a.N : a.K), (uint64_t)(a.kn ? a.K : a.N), (uint64_t)a.E};
   const uint32_t box_k[3] = {kb, 128, 1}, box_n[3] = {64, 64, 1};
-  if (int rc = encode_map(&maps.w, a.w, 3, dims, a.kn ? box_n : box_k, elem)) return rc;
+  if (int rc = encode_map(&maps.w, a.w, 3, dims, a.kn ? box_n : box_k, elem, (uint64_t)a.ldw * elem)) return rc;
   RowsParams p{};
   p.offsets = a.offsets; p.x_scale = a.x_scale; p.w_scale = a.w_scale; p.out = a.out;
   p.fault = device_fault_word();
@@ -721,23 +725,19 @@ int ragged_rows_tc(int elem, int out_dtype, const RaggedRows& a, cudaStream_t st
   return launch_rows<false, false, __nv_bfloat16>(maps, p, items, st);
 }
 
-bool ragged_wgrad_tc_takes(const RaggedWgrad& a) {
-  const uintptr_t bases = reinterpret_cast<uintptr_t>(a.a) | reinterpret_cast<uintptr_t>(a.b) | reinterpret_cast<uintptr_t>(a.out);
-  return a.R > 0 && a.P % 8 == 0 && a.Q % 8 == 0 && (bases & 15) == 0;
-}
-
 int ragged_wgrad_tc(const RaggedWgrad& a, cudaStream_t st) {
   CUtensorMap ma, mb;
   const uint32_t box[2] = {64, 64};
   const uint64_t da[2] = {(uint64_t)a.P, (uint64_t)a.R}, db[2] = {(uint64_t)a.Q, (uint64_t)a.R};
-  if (int rc = encode_map(&ma, a.a, 2, da, box, 2)) return rc;
-  if (int rc = encode_map(&mb, a.b, 2, db, box, 2)) return rc;
+  if (int rc = encode_map(&ma, a.a, 2, da, box, 2, (uint64_t)a.lda * 2)) return rc;
+  if (int rc = encode_map(&mb, a.b, 2, db, box, 2, (uint64_t)a.ldb * 2)) return rc;
   WgradParams p{};
   p.offsets = a.offsets;
   p.out = static_cast<__nv_bfloat16*>(a.out);
   p.fault = device_fault_word();
   MOLE_REQUIRE(p.fault != nullptr, "fault word not allocated");
   p.R = (int)a.R; p.P = a.P; p.Q = a.Q; p.E = a.E;
+  p.wide = a.Q % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
   constexpr size_t smem = (size_t)kWStages * kWStageBytes + 1024;
   static PerDeviceInt cache;
   int pairs = 0;

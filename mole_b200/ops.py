@@ -319,6 +319,21 @@ def _check_offsets(offsets: torch.Tensor, E: int) -> None:
         raise ValueError(f"offsets must be int32 [{E + 1}]")
 
 
+def _starts_on_16_bytes(t: torch.Tensor) -> bool:
+    return t.data_ptr() % 16 == 0 and t.shape[-1] * t.element_size() % 16 == 0
+
+
+def _mm_workspace(x: torch.Tensor, w: torch.Tensor, R: int, N: int, K: int, E: int, w_kn: bool):
+    """(tensor, address, bytes) of the copies that rows which do not start on 16 bytes need."""
+    if _starts_on_16_bytes(x) and _starts_on_16_bytes(w):
+        return None, None, 0
+    n = C.c_int64()
+    check(lib.mole_grouped_mm_workspace_bytes(x.data_ptr(), w.data_ptr(), R, N, K, E, int(w_kn), x.element_size(),
+                                              C.byref(n)))
+    ws = torch.empty(n.value, dtype=torch.uint8, device=x.device)
+    return ws, ws.data_ptr(), n.value
+
+
 def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, w_kn: bool = False,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``out[r] = x[r] @ w[e].T`` (``w`` ``[E, N, K]``), or ``x[r] @ w[e]`` with ``w_kn`` (``w``
@@ -337,8 +352,9 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, w_kn: bo
     elif out.shape != (x.shape[0], N) or out.dtype != x.dtype:
         raise ValueError(f"out must be {x.dtype} [{x.shape[0]}, {N}]")
     with _on_device_of(x, w, offsets, out):
+        ws, address, size = _mm_workspace(x, w, x.shape[0], N, K, E, w_kn)
         check(lib.mole_grouped_mm(_ptr(x), _ptr(w), _ptr(offsets), x.shape[0], N, K, E, int(w_kn), _dt(x),
-                                  _ptr(out), _stream()))
+                                  _ptr(out), address, size, _stream()))
     return out
 
 
@@ -357,8 +373,15 @@ def grouped_mm_wgrad(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor,
     elif out.shape != (E, P, Q) or out.dtype != a.dtype:
         raise ValueError(f"out must be {a.dtype} [{E}, {P}, {Q}]")
     with _on_device_of(a, b, offsets, out):
+        ws, size = None, 0
+        if not (_starts_on_16_bytes(a) and _starts_on_16_bytes(b)):
+            n = C.c_int64()
+            check(lib.mole_grouped_mm_wgrad_workspace_bytes(a.data_ptr(), b.data_ptr(), a.shape[0], P, Q, E, _dt(a),
+                                                            C.byref(n)))
+            size = n.value
+            ws = torch.empty(size, dtype=torch.uint8, device=a.device)
         check(lib.mole_grouped_mm_wgrad(_ptr(a), _ptr(b), _ptr(offsets), a.shape[0], P, Q, E, _dt(a),
-                                        _ptr(out), _stream()))
+                                        _ptr(out), _ptr(ws), size, _stream()))
     return out
 
 
@@ -393,8 +416,9 @@ def _mm_int8(q, q_scale, w, w_scale, offsets, E, N, K, out_dtype, out):
     elif out.shape != (R, N) or out.dtype != out_dtype:
         raise ValueError(f"out must be {out_dtype} [{R}, {N}]")
     with _on_device_of(q, q_scale, w, w_scale, offsets, out):
+        ws, address, size = _mm_workspace(q, w, R, N, K, E, False)
         check(lib.mole_grouped_mm_i8(_ptr(q), _ptr(q_scale), _ptr(w), _ptr(w_scale), _ptr(offsets), R, N, K, E,
-                                     _DTYPES[out_dtype], _ptr(out), _stream()))
+                                     _DTYPES[out_dtype], _ptr(out), address, size, _stream()))
     return out
 
 

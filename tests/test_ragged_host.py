@@ -18,9 +18,9 @@ def status(rc):
     (-1, 8, 8, 2, 1, -1), (1 << 31, 8, 8, 2, 1, -1), (10, 8, 8, 2, 7, -1), (0, 8, 8, 2, 1, 0)])
 def test_grouped_mm_sizes(R, N, K, E, dtype, code):
     from mole_b200 import _lib
-    assert _lib.lib.mole_grouped_mm(A, A, A, R, N, K, E, 0, dtype, A, None) == code
+    assert _lib.lib.mole_grouped_mm(A, A, A, R, N, K, E, 0, dtype, A, None, 0, None) == code
     if code:
-        assert _lib.lib.mole_grouped_mm_wgrad(A, A, A, R, N, K, E, dtype, A, None) == code
+        assert _lib.lib.mole_grouped_mm_wgrad(A, A, A, R, N, K, E, dtype, A, None, 0, None) == code
 
 
 def test_null_and_misaligned_pointers():
@@ -29,25 +29,53 @@ def test_null_and_misaligned_pointers():
     for bad in range(4):
         p = [A] * 4
         p[bad] = None
-        assert status(lib.mole_grouped_mm(p[0], p[1], p[2], 4, 8, 8, 2, 0, 1, p[3], None)) == (-1, "null pointer argument")
+        assert status(lib.mole_grouped_mm(p[0], p[1], p[2], 4, 8, 8, 2, 0, 1, p[3], None, 0, None)) == (-1, "null pointer argument")
         p[bad] = A + 1
-        rc, text = status(lib.mole_grouped_mm(p[0], p[1], p[2], 4, 8, 8, 2, 0, 1, p[3], None))
+        rc, text = status(lib.mole_grouped_mm(p[0], p[1], p[2], 4, 8, 8, 2, 0, 1, p[3], None, 0, None))
         assert rc == -1 and "aligned" in text
-    assert lib.mole_grouped_mm_wgrad(A, A, None, 0, 8, 8, 2, 1, A, None) == -1
+    assert lib.mole_grouped_mm_wgrad(A, A, None, 0, 8, 8, 2, 1, A, None, 0, None) == -1
     assert lib.mole_quantize_rows(None, 3, 8, 1, A, A, None) == -1
     assert lib.mole_quantize_rows(A, 3, 0, 1, A, A, None) == -1
     assert lib.mole_quantize_rows(A, 0, 8, 1, A, A, None) == 0
 
 
+def test_workspace_of_rows_that_do_not_start_on_16_bytes():
+    from mole_b200 import _lib
+    lib = _lib.lib
+    n = C.c_int64()
+
+    def size(x, w, R, N, K, E, kn, elem):
+        assert lib.mole_grouped_mm_workspace_bytes(x, w, R, N, K, E, kn, elem, C.byref(n)) == 0
+        return n.value
+    up = lambda b: -(-b // 256) * 256  # noqa: E731
+    assert size(A, A, 100, 33, 64, 3, 0, 2) == 0                 # only the reduction has to fit
+    assert size(A, A, 100, 33, 64, 3, 1, 2) == up(3 * 64 * 40 * 2)
+    assert size(A, A, 100, 64, 33, 3, 1, 2) == up(100 * 40 * 2)
+    assert size(A, A, 100, 64, 33, 3, 0, 2) == up(100 * 40 * 2) + up(3 * 64 * 40 * 2)
+    assert size(A + 2, A, 100, 64, 64, 3, 0, 2) == up(100 * 64 * 2)
+    assert size(A, A, 100, 64, 24, 3, 0, 1) == up(100 * 32) + up(3 * 64 * 32)
+    assert size(A, A, 16, 64, 33, 3, 0, 2) == 0 and size(A, A, 100, 64, 33, 3, 0, 4) == 0
+    assert lib.mole_grouped_mm_workspace_bytes(A, A, 100, 64, 33, 3, 0, 3, C.byref(n)) == -1
+    assert lib.mole_grouped_mm_wgrad_workspace_bytes(A, A, 100, 64, 33, 3, 1, C.byref(n)) == 0
+    assert n.value == up(100 * 40 * 2)
+    # too little of it
+    rc, text = status(lib.mole_grouped_mm(A, A, A, 100, 64, 33, 3, 0, 1, A, None, 0, None))
+    assert rc == -1 and "workspace" in text
+    rc, text = status(lib.mole_grouped_mm_wgrad(A, A, A, 100, 64, 33, 3, 1, A, A, 100, None))
+    assert rc == -1 and "workspace" in text
+    rc, text = status(lib.mole_grouped_mm_i8(A, A, A, A, A, 100, 64, 24, 3, 0, A, A, 100, None))
+    assert rc == -1 and "workspace" in text
+
+
 def test_integer_products():
     from mole_b200 import _lib
     lib = _lib.lib
-    rc, text = status(lib.mole_grouped_mm_i8(A, A, A, A, A, 4, 8, 1 << 17, 1, 0, A, None))
+    rc, text = status(lib.mole_grouped_mm_i8(A, A, A, A, A, 4, 8, 1 << 17, 1, 0, A, None, 0, None))
     assert rc == -1 and "32 bits" in text
-    rc, text = status(lib.mole_grouped_mm_i8(A, A, A, A, None, 4, 8, 16, 2, 0, A, None))
+    rc, text = status(lib.mole_grouped_mm_i8(A, A, A, A, None, 4, 8, 16, 2, 0, A, None, 0, None))
     assert rc == -1 and "one expert" in text
-    assert lib.mole_grouped_mm_i8(A, None, A, A, A, 4, 8, 16, 2, 0, A, None) == -1
-    assert lib.mole_grouped_mm_i8(A, A, A, A, None, 0, 8, 16, 1, 0, A, None) == 0
+    assert lib.mole_grouped_mm_i8(A, None, A, A, A, 4, 8, 16, 2, 0, A, None, 0, None) == -1
+    assert lib.mole_grouped_mm_i8(A, A, A, A, None, 0, 8, 16, 1, 0, A, None, 0, None) == 0
 
 
 def test_adam_list():
