@@ -8,10 +8,11 @@ namespace mole {
 
 // ---- rows to 8-bit integers ------------------------------------------------------------------
 // scale = max |x| / 127 rounded to fp32; q = the integer nearest to x / scale, ties to even.  The
-// quotient is taken as x * (1 / scale), which is off by less than 2^-23 of 127; where that leaves
+// quotient t is taken as x * (1 / scale), which is off by less than 2^-23 of 127; where that leaves
 // doubt about the nearest integer (1 value in 10^4), the sign of x - (n + 1/2) scale decides, which
-// one fused multiply-add gives exactly.
-__device__ __forceinline__ int quantize_one(float x, float scale, float inv) {
+// one fused multiply-add gives exactly.  (A call: inlined 64 times, the kernel misses in the instruction
+// cache.)
+__device__ __noinline__ int quantize_one(float x, float scale, float inv) {
   const float t = x * inv;
   float r = rintf(t);
   if (fabsf(fabsf(t - r) - 0.5f) < 6e-5f) {
@@ -25,7 +26,6 @@ __device__ __forceinline__ int quantize_one(float x, float scale, float inv) {
 // One row per group of G threads (a warp or a block).  HELD: the row fits the group's registers (eight
 // 16-byte vectors a thread), is read once and waits there for its scale; otherwise it is read twice.
 // V = 1: rows that 16-byte loads cannot address.
-// Bound by HBM (3 bytes an element of bf16): 32768 x 2048 in 41 us, 4.9 TB/s.
 template <typename T, int V, int G, bool HELD>
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const T* __restrict__ x, int64_t R, int K, int8_t* __restrict__ q, float* __restrict__ scale) {
@@ -77,17 +77,32 @@ quantize_rows_kernel(const T* __restrict__ x, int64_t R, int K, int8_t* __restri
   // rows of tiny values: both sides times 2^100, so that neither 1 / scale overflows nor the
   // difference in quantize_one leaves the range of fp32
   const float up = s < 0x1p-100f ? 0x1p100f : 1.f;
+  const bool odd = zero || s < 0x1p-100f;
   const float su = s * up, inv = zero ? 0.f : __fdiv_rn(1.f, su);
   auto store = [&](int k, const float (&v)[V]) {
-    uint32_t w[(V + 3) / 4] = {};
+    uint32_t w[V];
+    float off[V], doubt = 0.f;
+    // the nearest integer sits in the low bits of t + 3 2^22 (|t| rounds to 127 at most); a quotient in
+    // doubt is nearly half a unit off it.  bf16 rows are full of true ties (both x and the top have 8 bits):
+    // one element in some hundred, looked at one by one.
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int n = zero ? 0 : quantize_one(v[i] * up, su, inv);
-      w[i >> 2] |= ((uint32_t)n & 0xffu) << (8 * (i & 3));
+      const float t = v[i] * inv, r = t + 12582912.f;
+      w[i] = __float_as_uint(r);
+      off[i] = fabsf(t - (r - 12582912.f));
+      doubt = fmaxf(doubt, off[i]);
+    }
+    if (doubt > 0.5f - 6e-5f || odd) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (off[i] > 0.5f - 6e-5f || odd) w[i] = zero ? 0u : (uint32_t)quantize_one(v[i] * up, su, inv);
     }
     int8_t* d = q + row * K + k;
-    if constexpr (V == 8) *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
-    else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(d) = w[0];
+    auto pack = [](uint32_t a, uint32_t b, uint32_t c, uint32_t e) {
+      return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, e, 0x0040), 0x5410);
+    };
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(d) = make_uint2(pack(w[0], w[1], w[2], w[3]), pack(w[4], w[5], w[6], w[7]));
+    else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(d) = pack(w[0], w[1], w[2], w[3]);
     else *d = (int8_t)w[0];
   };
   if constexpr (HELD) {
