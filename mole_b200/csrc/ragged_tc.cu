@@ -515,7 +515,7 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull0 + 8 * a, 1);
-      mbar_init(tempty0 + 8 * a, 2 * kREpiWarps);
+      mbar_init(tempty0 + 8 * a, kREpiWarps);       // eight warps of either CTA
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -630,72 +630,85 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       if (lane == 0) mbar_arrive_release_cluster((full0 + 8 * last) & kPeerMask);
     }
   } else if (warp >= 4) {
-    // ---- epilogue (both CTAs): warp -> 32 rows of the gradient, 64 columns ----
-    const int quarter = warp & 3, grp = (warp - 4) >> 2;
+    // ---- epilogue (both CTAs): warp -> 32 rows of the gradient and 128 columns of every second item ----
+    // (the two accumulators have eight warps each: a warp's way from TMEM to memory takes longer than an
+    // item's MMAs, and so two of them are under way)
+    const int quarter = warp & 3, grp = ((warp - 4) >> 2) & 1, acc = (warp - 4) >> 3;
     uint8_t* strip = reinterpret_cast<uint8_t*>(strips[warp - 4]);
-    int acc = 0;
+    int turn = 0;
     uint32_t acc_phase = 0;
     for (int item = cluster_id;; item += n_clusters) {
       const WgradItem w = wgrad_item(ord, p, item);
       if (!w.valid) break;
       const bool empty = w.rows == 0;               // no rows: the gradient is zero
+      if (empty ? ((item / n_clusters) & 1) != acc : turn != acc) {
+        if (!empty) turn ^= 1;
+        continue;
+      }
       if (!empty) {
+        turn ^= 1;
         if (!warp_all_wait(tfull0 + 8 * acc, acc_phase, abort_flag, p.fault, 75)) break;
         tcgen05_fence_after();
+        acc_phase ^= 1;
       }
       const int prow = w.p0 + 128 * (int)rank + 32 * quarter;     // of lane 0
-      const int qcol = w.q0 + 64 * grp;
-      const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + 256 * acc + 64 * grp;
-      uint32_t o[4][8];
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        uint32_t r[16];
+#pragma unroll 1
+      for (int part = 0; part < 2; ++part) {
+        const int col = 128 * grp + 64 * part, qcol = w.q0 + col;
+        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + 256 * acc + col;
+        uint32_t o[4][8];
         if (!empty) {
-          tmem_ld16(taddr + 16 * s, r);
+          uint32_t r[4][16];
+#pragma unroll
+          for (int s = 0; s < 4; ++s) tmem_ld16(taddr + 16 * s, r[s]);
           tmem_ld_wait();
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) r[i] = 0u;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[s][i] = two_bf16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-      }
-      if (!empty) {
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster((tempty0 + 8 * acc) & kPeerMask);
-        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
-      }
-      // through the strip in four passes of eight rows (128 bytes each), 16-byte pieces swizzled by the
-      // row: a store instruction then writes whole 128-byte lines
-      __nv_bfloat16* out = p.out + ((int64_t)w.e * p.P + prow) * p.Q + qcol;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        __syncwarp();
-        if ((lane >> 3) == j) {
-          const int rr = lane & 7;
 #pragma unroll
           for (int s = 0; s < 4; ++s)
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf)
-              *reinterpret_cast<uint4*>(strip + rr * 128 + (((2 * s + hf) ^ rr) << 4)) =
-                  make_uint4(o[s][4 * hf], o[s][4 * hf + 1], o[s][4 * hf + 2], o[s][4 * hf + 3]);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int rr = (lane >> 3) + 4 * k, piece = lane & 7;
-          const uint4 v = *reinterpret_cast<const uint4*>(strip + rr * 128 + ((piece ^ rr) << 4));
-          if (prow + 8 * j + rr >= p.P) continue;
-          __nv_bfloat16* d = out + (int64_t)(8 * j + rr) * p.Q + 8 * piece;
-          const int left = p.Q - qcol - 8 * piece;
-          if (p.wide) {
-            if (left > 0) *reinterpret_cast<uint4*>(d) = v;
-          } else {
-            const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&v);
-#pragma unroll
             for (int i = 0; i < 8; ++i)
-              if (i < left) d[i] = b[i];
+              o[s][i] = two_bf16(__uint_as_float(r[s][2 * i]), __uint_as_float(r[s][2 * i + 1]));
+          if (part == 1) {
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster((tempty0 + 8 * acc) & kPeerMask);
+          }
+        } else {
+#pragma unroll
+          for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[s][i] = 0u;
+        }
+        // through the strip in four passes of eight rows (128 bytes each), 16-byte pieces swizzled by the
+        // row: a store instruction then writes whole 128-byte lines
+        __nv_bfloat16* out = p.out + ((int64_t)w.e * p.P + prow) * p.Q + qcol;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          __syncwarp();
+          if ((lane >> 3) == j) {
+            const int rr = lane & 7;
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+              for (int hf = 0; hf < 2; ++hf)
+                *reinterpret_cast<uint4*>(strip + rr * 128 + (((2 * s + hf) ^ rr) << 4)) =
+                    make_uint4(o[s][4 * hf], o[s][4 * hf + 1], o[s][4 * hf + 2], o[s][4 * hf + 3]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int rr = (lane >> 3) + 4 * k, piece = lane & 7;
+            const uint4 v = *reinterpret_cast<const uint4*>(strip + rr * 128 + ((piece ^ rr) << 4));
+            if (prow + 8 * j + rr >= p.P) continue;
+            __nv_bfloat16* d = out + (int64_t)(8 * j + rr) * p.Q + 8 * piece;
+            const int left = p.Q - qcol - 8 * piece;
+            if (p.wide) {
+              if (left > 0) *reinterpret_cast<uint4*>(d) = v;
+            } else {
+              const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&v);
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (i < left) d[i] = b[i];
+            }
           }
         }
       }
