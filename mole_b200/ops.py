@@ -2,13 +2,12 @@
 
 PyTorch owns device memory and streams; every function here checks shapes, allocates outputs
 with ``torch.empty`` and hands raw pointers to ``libmole_b200.so`` on the current stream.
-None of them has a PyTorch fallback.
+None of them has a PyTorch fallback.  The products over packed rows and the Adam step over many tensors
+do the same in ``_host.so``, on the current stream of their tensors' device.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
-import itertools
 import math
 from dataclasses import dataclass
 from typing import Optional, Sequence
@@ -16,7 +15,8 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from ._lib import AdamTensor, FfnDesc, check, lib
+from ._host import host
+from ._lib import FfnDesc, check, lib
 
 _DTYPES = {torch.float32: _lib.MOLE_F32, torch.bfloat16: _lib.MOLE_BF16}
 _ACTS = {"gelu": _lib.ACT_GELU, "relu": _lib.ACT_RELU}
@@ -44,19 +44,6 @@ def _stream() -> int:
     # the raw handle of the current stream of the current device; torch.cuda.current_stream()
     # builds a Stream object through several Python layers (17 us a call, a dozen calls a step)
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
-
-
-def _on_device_of(first: torch.Tensor, *others: Optional[torch.Tensor]):
-    """Context in which the current device is the one all these tensors are on."""
-    dev = first.device
-    if dev.type != "cuda":
-        raise RuntimeError("mole_b200 kernels take CUDA tensors only (there is no CPU path)")
-    for t in others:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors are on different devices: {dev} and {t.device}")
-    if dev.index == torch._C._cuda_getDevice():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
 
 
 def capacity(T: int, E: int, k: int, capacity_factor: float) -> int:
@@ -314,112 +301,26 @@ def ffn_bwd_peer(desc: FfnDesc, counts, dout, x, x1, h, w1, w2, dx1, peer, gw1, 
 
 
 # ---- products over rows packed by expert --------------------------------------------------------
-def _check_offsets(offsets: torch.Tensor, E: int) -> None:
-    if offsets.dtype != torch.int32 or offsets.shape != (E + 1,):
-        raise ValueError(f"offsets must be int32 [{E + 1}]")
-
-
-def _starts_on_16_bytes(t: torch.Tensor) -> bool:
-    return t.data_ptr() % 16 == 0 and t.shape[-1] * t.element_size() % 16 == 0
-
-
-def _mm_workspace(x: torch.Tensor, w: torch.Tensor, R: int, N: int, K: int, E: int, w_kn: bool):
-    """(tensor, address, bytes) of the copies that rows which do not start on 16 bytes need."""
-    if _starts_on_16_bytes(x) and _starts_on_16_bytes(w):
-        return None, None, 0
-    n = C.c_int64()
-    check(lib.mole_grouped_mm_workspace_bytes(x.data_ptr(), w.data_ptr(), R, N, K, E, int(w_kn), x.element_size(),
-                                              C.byref(n)))
-    ws = torch.empty(n.value, dtype=torch.uint8, device=x.device)
-    return ws, ws.data_ptr(), n.value
-
-
 def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, w_kn: bool = False,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``out[r] = x[r] @ w[e].T`` (``w`` ``[E, N, K]``), or ``x[r] @ w[e]`` with ``w_kn`` (``w``
     ``[E, K, N]``), for the rows ``offsets[e] <= r < offsets[e + 1]`` of every expert.  ``offsets``
     (int32 ``[E + 1]``, ``RoutePlan.offsets``) stays on the device; rows of no expert become zeros."""
-    if x.dim() != 2 or w.dim() != 3:
-        raise ValueError("grouped_mm takes x [R, K] and w [E, N, K] or [E, K, N]")
-    E, N, K = w.shape[0], w.shape[2 if w_kn else 1], w.shape[1 if w_kn else 2]
-    if x.shape[1] != K:
-        raise ValueError(f"x has width {x.shape[1]}, the weights take {K}")
-    if w.dtype != x.dtype:
-        raise TypeError("x and w must have one dtype")
-    _check_offsets(offsets, E)
-    if out is None:
-        out = torch.empty(x.shape[0], N, dtype=x.dtype, device=x.device)
-    elif out.shape != (x.shape[0], N) or out.dtype != x.dtype:
-        raise ValueError(f"out must be {x.dtype} [{x.shape[0]}, {N}]")
-    with _on_device_of(x, w, offsets, out):
-        ws, address, size = _mm_workspace(x, w, x.shape[0], N, K, E, w_kn)
-        check(lib.mole_grouped_mm(_ptr(x), _ptr(w), _ptr(offsets), x.shape[0], N, K, E, int(w_kn), _dt(x),
-                                  _ptr(out), address, size, _stream()))
-    return out
+    return host.grouped_mm(x, w, offsets, w_kn, out)
 
 
 def grouped_mm_wgrad(a: torch.Tensor, b: torch.Tensor, offsets: torch.Tensor,
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``out[e] = a_e.T @ b_e`` over the rows of every expert: ``[E, P, Q]`` from ``a [R, P]`` and
     ``b [R, Q]``; zeros for an expert without rows."""
-    if a.dim() != 2 or b.dim() != 2 or a.shape[0] != b.shape[0]:
-        raise ValueError("grouped_mm_wgrad takes a [R, P] and b [R, Q]")
-    if a.dtype != b.dtype:
-        raise TypeError("a and b must have one dtype")
-    E, P, Q = offsets.numel() - 1, a.shape[1], b.shape[1]
-    _check_offsets(offsets, E)
-    if out is None:
-        out = torch.empty(E, P, Q, dtype=a.dtype, device=a.device)
-    elif out.shape != (E, P, Q) or out.dtype != a.dtype:
-        raise ValueError(f"out must be {a.dtype} [{E}, {P}, {Q}]")
-    with _on_device_of(a, b, offsets, out):
-        ws, size = None, 0
-        if not (_starts_on_16_bytes(a) and _starts_on_16_bytes(b)):
-            n = C.c_int64()
-            check(lib.mole_grouped_mm_wgrad_workspace_bytes(a.data_ptr(), b.data_ptr(), a.shape[0], P, Q, E, _dt(a),
-                                                            C.byref(n)))
-            size = n.value
-            ws = torch.empty(size, dtype=torch.uint8, device=a.device)
-        check(lib.mole_grouped_mm_wgrad(_ptr(a), _ptr(b), _ptr(offsets), a.shape[0], P, Q, E, _dt(a),
-                                        _ptr(out), _ptr(ws), size, _stream()))
-    return out
+    return host.grouped_mm_wgrad(a, b, offsets, out)
 
 
 def quantize_rows(x: torch.Tensor):
     """``(q int8, scale float32)``: every row (last dimension) of ``x`` in 8-bit integers with one
     scale, ``q = round(x / scale)``, ``scale = max|row| / 127``.  Used for tokens (``[R, K]``) and, once, for
     weights ``[E, N, K]``, whose rows are the output channels."""
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError("quantize_rows needs rows of at least one element")
-    K = x.shape[-1]
-    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    with _on_device_of(x):
-        check(lib.mole_quantize_rows(_ptr(x), scale.numel(), K, _dt(x), _ptr(q), _ptr(scale), _stream()))
-    return q, scale
-
-
-def _mm_int8(q, q_scale, w, w_scale, offsets, E, N, K, out_dtype, out):
-    if q.dtype != torch.int8 or w.dtype != torch.int8:
-        raise TypeError("the operands must be int8")
-    if q.dim() != 2 or q.shape[1] != K:
-        raise ValueError(f"q must be [R, {K}]")
-    R = q.shape[0]
-    if q_scale.dtype != torch.float32 or q_scale.shape != (R,):
-        raise ValueError(f"q_scale must be float32 [{R}]")
-    if w_scale.dtype != torch.float32 or w_scale.shape != w.shape[:-1]:
-        raise ValueError(f"w_scale must be float32 {list(w.shape[:-1])}")
-    if out_dtype not in _DTYPES:
-        raise TypeError(f"unsupported dtype {out_dtype}; the kernels cover float32 and bfloat16")
-    if out is None:
-        out = torch.empty(R, N, dtype=out_dtype, device=q.device)
-    elif out.shape != (R, N) or out.dtype != out_dtype:
-        raise ValueError(f"out must be {out_dtype} [{R}, {N}]")
-    with _on_device_of(q, q_scale, w, w_scale, offsets, out):
-        ws, address, size = _mm_workspace(q, w, R, N, K, E, False)
-        check(lib.mole_grouped_mm_i8(_ptr(q), _ptr(q_scale), _ptr(w), _ptr(w_scale), _ptr(offsets), R, N, K, E,
-                                     _DTYPES[out_dtype], _ptr(out), address, size, _stream()))
-    return out
+    return host.quantize_rows(x)
 
 
 def grouped_mm_int8(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
@@ -428,20 +329,15 @@ def grouped_mm_int8(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_s
     """``grouped_mm`` of 8-bit integers: ``out[r, n] = (q[r] . w[e, n]) * q_scale[r] * w_scale[e, n]`` with
     ``q [R, K]``, ``w [E, N, K]`` int8 (``quantize_rows`` of the tokens and of the weights), the sum of
     products exact."""
-    if w.dim() != 3:
-        raise ValueError("grouped_mm_int8 takes w [E, N, K]")
-    E, N, K = w.shape
-    _check_offsets(offsets, E)
-    return _mm_int8(q, q_scale, w, w_scale, offsets, E, N, K, out_dtype, out)
+    if offsets is None:
+        raise TypeError("grouped_mm_int8 takes offsets; mm_int8 is the product with one matrix for all rows")
+    return host.mm_int8(q, q_scale, w, w_scale, offsets, out_dtype, out)
 
 
 def mm_int8(q: torch.Tensor, q_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
             out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The same product with one weight matrix ``w [N, K]`` for all rows."""
-    if w.dim() != 2:
-        raise ValueError("mm_int8 takes w [N, K]")
-    N, K = w.shape
-    return _mm_int8(q, q_scale, w, w_scale, None, 1, N, K, out_dtype, out)
+    return host.mm_int8(q, q_scale, w, w_scale, None, out_dtype, out)
 
 
 # ---- one Adam step over many tensors ---------------------------------------------------------
@@ -467,53 +363,8 @@ def adam_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     ``v = (code * scale) ** 2``; zeros are a fresh state).  8-bit moments are rounded at random by
     bits that ``seed``, ``t``, the place in the list and the element determine: the same call gives
     the same bits."""
-    lists = [params, grads, exp_avgs, exp_avg_sqs]
-    n = len(params)
-    if n == 0:
-        return
-    bits = 8 if exp_avgs[0].dtype == torch.float8_e4m3fn else 32
-    if bits == 8:
-        if m_scales is None or v_scales is None:
-            raise ValueError("8-bit moments need m_scales and v_scales")
-        lists += [m_scales, v_scales]
-    elif m_scales is not None or v_scales is not None:
-        raise ValueError("32-bit moments have no scales")
-    if any(len(x) != n for x in lists):
-        raise ValueError("one gradient, two moments (and their scales) per parameter")
-    dt = _dt(params[0])
-    # The checks run list by list over C-level methods: a step over hundreds of small tensors takes no
-    # longer on the GPU than on the host.
-    dtype, index = params[0].dtype, params[0].get_device()
-    if not params[0].is_cuda:
-        raise RuntimeError("mole_b200 kernels take CUDA tensors only (there is no CPU path)")
-    if any(set(map(torch.Tensor.get_device, xs)) != {index} for xs in lists):
-        raise ValueError("the tensors are on different devices")
-    mdtype = torch.float8_e4m3fn if bits == 8 else torch.float32
-    for xs, want, what in zip(lists, (dtype, dtype, mdtype, mdtype, torch.float32, torch.float32),
-                              ("parameters", "gradients", "moments", "moments", "scales", "scales")):
-        if {x.dtype for x in xs} != {want}:
-            raise TypeError(f"the {what} must all be {want}")
-        if not all(map(torch.Tensor.is_contiguous, xs)):
-            raise RuntimeError("mole_b200 kernels take contiguous tensors")
-    sizes = list(map(torch.Tensor.numel, params))
-    if any(list(map(torch.Tensor.numel, xs)) != sizes for xs in lists[1:4]):
-        raise ValueError("parameters, gradients and moments differ in size")
-    if bits == 8:
-        blocks = [-(-k // ADAM_BLOCK) for k in sizes]
-        if any(list(map(torch.Tensor.numel, xs)) != blocks for xs in lists[4:]):
-            raise ValueError(f"scales must be float32, one per {ADAM_BLOCK} elements")
-    columns = [list(map(torch.Tensor.data_ptr, xs)) for xs in lists]
-    held = [q for q in columns[0] if q]
-    if len(set(held)) != len(held):
-        raise ValueError("the same parameter twice in one call")
-    if bits == 32:
-        columns += [[0] * n] * 2
-    words = (C.c_uint64 * (7 * n))(*itertools.chain.from_iterable(zip(*columns, sizes)))
-    table = C.cast(words, C.POINTER(AdamTensor))
-    with _on_device_of(params[0]):
-        check(lib.mole_adam_multi(table, n, dt, bits, betas[0], betas[1], int(t), float(lr),
-                                  float(weight_decay), float(eps), int(bool(adamw)),
-                                  int(seed) & 0xffffffff, _stream()))
+    host.adam_multi(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales, t, lr, betas[0], betas[1], eps,
+                    weight_decay, adamw, seed)
 
 
 def device_fault_poll() -> None:
