@@ -16,9 +16,8 @@
 // The tensors' table travels in the launch's parameters: no copy to the device, nothing to keep
 // alive, and the launch can be issued on any stream.
 //
-// Which products and sums share a rounding is written out (fused multiply-adds by name, in both forms
-// of the arithmetic below): whether a state's code is the one above or below must not depend on how
-// a compiler contracts.
+// Every product, sum, quotient and root is rounded by itself, in both forms of the arithmetic below:
+// whether a state's code is the one above or below must not depend on how a compiler contracts.
 #include <cuda_fp8.h>
 
 #include <cmath>
@@ -54,6 +53,7 @@ struct AdamTable {
 struct AdamMulti {
   float decay, lam;        // AdamW: decay = 1 - lr lam, lam = 0; Adam: decay = 1, lam
   float b1, c1, b2, c2, step, r2, eps;
+  float one;               // 1, which the compiler must not know
   uint32_t key;            // of (seed, t)
   int chunks;              // of all entries; a thread block walks every gridDim.x-th
   int n_entries;
@@ -219,11 +219,11 @@ __device__ __noinline__ void adam_block(const AdamEntry& e, const AdamMulti& a, 
   float s[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    if (a.lam != 0.f) g[i] = __fmaf_rn(a.lam, p[i], g[i]);
-    m[i] = __fmaf_rn(a.b1, m[i], __fmul_rn(a.c1, g[i]));
-    v[i] = __fmaf_rn(a.b2, v[i], __fmul_rn(__fmul_rn(a.c2, g[i]), g[i]));
+    if (a.lam != 0.f) g[i] = __fadd_rn(g[i], __fmul_rn(a.lam, p[i]));
+    m[i] = __fadd_rn(__fmul_rn(a.b1, m[i]), __fmul_rn(a.c1, g[i]));
+    v[i] = __fadd_rn(__fmul_rn(a.b2, v[i]), __fmul_rn(__fmul_rn(a.c2, g[i]), g[i]));
     s[i] = __fsqrt_rn(v[i]);
-    p[i] = __fmaf_rn(p[i], a.decay, -__fdiv_rn(__fmul_rn(a.step, m[i]), __fmaf_rn(s[i], a.r2, a.eps)));
+    p[i] = __fsub_rn(__fmul_rn(p[i], a.decay), __fdiv_rn(__fmul_rn(a.step, m[i]), __fadd_rn(__fmul_rn(s[i], a.r2), a.eps)));
   }
   adam_store8(pp, n, wide, p);
   if (BITS == 32) {
@@ -348,13 +348,13 @@ __device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c
 
 // The scalars of the whole blocks' form, twice each where pairs take them
 struct AdamConsts {
-  uint64_t lam2, b12, c12, b22, c22, decay2;
+  uint64_t lam2, b12, c12, b22, c22, decay2, one2;
   float step, r2, eps;
   bool l2;
   __device__ __forceinline__ void init(const AdamMulti& a) {
     lam2 = f2_dup(a.lam);
     l2 = a.lam != 0.f;
-    b12 = f2_dup(a.b1); c12 = f2_dup(a.c1); b22 = f2_dup(a.b2); c22 = f2_dup(a.c2); decay2 = f2_dup(a.decay);
+    b12 = f2_dup(a.b1); c12 = f2_dup(a.c1); b22 = f2_dup(a.b2); c22 = f2_dup(a.c2); decay2 = f2_dup(a.decay); one2 = f2_dup(a.one);
     step = a.step; r2 = a.r2; eps = a.eps;
   }
 };
@@ -387,18 +387,19 @@ __device__ __forceinline__ bool adam_block_full(uint8_t* stage, int b, float2& s
       v[i] = f2_mul(v[i], f2_dup(scale.y));
       v[i] = f2_mul(v[i], v[i]);
     }
-    if (a.l2) g = f2_fma(a.lam2, p[i], g);
-    m[i] = f2_fma(a.b12, m[i], f2_mul(a.c12, g));
-    v[i] = f2_fma(a.b22, v[i], f2_mul(f2_mul(a.c22, g), g));
+    // x + y as x * one + y: the compiler contracts packed products into packed sums that follow them
+    if (a.l2) g = f2_fma(f2_mul(a.lam2, p[i]), a.one2, g);
+    m[i] = f2_fma(f2_mul(a.b12, m[i]), a.one2, f2_mul(a.c12, g));
+    v[i] = f2_fma(f2_mul(a.b22, v[i]), a.one2, f2_mul(f2_mul(a.c22, g), g));
     float v0, v1, m0, m1;
     f2_unpack(v[i], v0, v1);
     f2_unpack(m[i], m0, m1);
     const float s0 = root(v0), s1 = root(v1);
     s[i] = f2_pack(s0, s1);
-    const uint64_t q = f2_pack(minus_quotient(__fmul_rn(a.step, m0), __fmaf_rn(s0, a.r2, a.eps)),
-                               minus_quotient(__fmul_rn(a.step, m1), __fmaf_rn(s1, a.r2, a.eps)));
+    const uint64_t q = f2_pack(minus_quotient(__fmul_rn(a.step, m0), __fadd_rn(__fmul_rn(s0, a.r2), a.eps)),
+                               minus_quotient(__fmul_rn(a.step, m1), __fadd_rn(__fmul_rn(s1, a.r2), a.eps)));
     sum = i == 0 ? q : f2_add(sum, q);
-    p[i] = f2_fma(p[i], a.decay2, q);
+    p[i] = f2_fma(f2_mul(p[i], a.decay2), a.one2, q);
   }
   float lo, hi;
   f2_unpack(sum, lo, hi);
@@ -716,6 +717,7 @@ extern "C" int mole_adam_multi(const mole_adam_tensor* tensors, int32_t n_tensor
   a.step = (float)(lr / (1.0 - std::pow(beta1, (double)t)));
   a.r2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)t)));
   a.eps = (float)eps;
+  a.one = 1.f;
   a.key = adam_mix(adam_mix(seed) + (uint32_t)t);
   if (dtype == MOLE_F32)
     return state_bits == 32 ? adam_all<float, 32>(tensors, n_tensors, a, st) : adam_all<float, 8>(tensors, n_tensors, a, st);

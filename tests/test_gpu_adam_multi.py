@@ -2,11 +2,11 @@
 ``MOLEMixedAdam(state_bits=...)``).
 
 The 32-bit form is compared with the formula in 64 bits, and every state and parameter with the same
-operations in numpy's float32 (a fused multiply-add is the sum in 64 bits, rounded once): the
-rounding of an 8-bit state up or down depends on every bit, so nothing less says whether a code is
-right.  All bits have to be equal, but for one value in a thousand that may be one unit of fp32 off (the
-root and the quotient are correctly rounded but for about one in 2^20, and so is the sum in 64
-bits) and, where that moves a value across its random threshold, one code."""
+operations in numpy's float32, each rounded by itself: the rounding of an 8-bit state up or down
+depends on every bit, so nothing less says whether a code is right.  All bits have to be equal, but
+for one value in a thousand that may be one unit of fp32 off (the kernel's root and quotient are
+correctly rounded but for about one in 2^20) and, where that moves a value across its random
+threshold, one code."""
 import copy
 import math
 
@@ -71,14 +71,14 @@ def step_f32(p, g, m, v, t, place, adamw, seed, bits, ms=None, vs=None):
         m = m * rep(ms)
         v = v * rep(vs)
         v = v * v
-    fma = lambda a, b, c: (np.asarray(a, np.float64) * b + c).astype(f32)  # noqa: E731
     if not adamw:
-        g = fma(f32(lam), p, g)
-    m = fma(f32(b1), m, f32(1 - b1) * g)
-    v = fma(f32(b2), v, (f32(1 - b2) * g) * g)
+        g = g + f32(lam) * p
+    m = f32(b1) * m + f32(1 - b1) * g
+    v = f32(b2) * v + (f32(1 - b2) * g) * g
     s = np.sqrt(v)
-    q = (f32(lr / (1 - b1 ** t)) * m) / fma(s, f32(1 / math.sqrt(1 - b2 ** t)), f32(eps))
-    p = fma(p, f32(1 - lr * lam) if adamw else f32(1), -q)
+    if adamw:
+        p = p * f32(1 - lr * lam)
+    p = p - (f32(lr / (1 - b1 ** t)) * m) / (s * f32(1 / math.sqrt(1 - b2 ** t)) + f32(eps))
     if bits == 32:
         return p, m, v, None, None
     w = random_words(n, seed, t, place)
