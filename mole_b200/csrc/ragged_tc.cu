@@ -451,6 +451,7 @@ constexpr int kWStages = 6;
 constexpr uint32_t kWHalfBytes = 128 * 128;              // 128 columns x 64 rows of one operand, two boxes
 constexpr uint32_t kWStageBytes = 2 * kWHalfBytes;
 constexpr uint32_t kWBoxBytes = 64 * 128;                // 64 columns x 64 rows
+constexpr uint32_t kWStripBytes = 32 * 64;               // per epilogue warp: 32 rows x 32 columns on their way out
 
 struct WgradParams {
   const int32_t* offsets;
@@ -459,10 +460,14 @@ struct WgradParams {
   int R, P, Q, E;
   int wide;             // rows of out are multiples of 16 bytes, its base too
 };
+struct WgradOrder {
+  int row0[kMaxRaggedExperts + 3];
+  uint8_t order[kMaxRaggedExperts];      // experts by falling row counts
+};
 struct WgradItem {
   int valid, e, p0, q0, row0, rows;
 };
-__device__ __forceinline__ WgradItem wgrad_item(const RowsOrder& o, const WgradParams& p, int item) {
+__device__ __forceinline__ WgradItem wgrad_item(const WgradOrder& o, const WgradParams& p, int item) {
   WgradItem w;
   const int qb = (p.Q + 255) / 256, per = (p.P + 255) / 256 * qb;
   w.valid = item < p.E * per;
@@ -478,7 +483,7 @@ __device__ __forceinline__ WgradItem wgrad_item(const RowsOrder& o, const WgradP
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kRThreads, 1)
 ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                       const __grid_constant__ WgradParams p) {
+                       const __grid_constant__ CUtensorMap map_out, const __grid_constant__ WgradParams p) {
   constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) |
                               ((uint32_t)(256 >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
   extern __shared__ uint8_t smem_raw[];
@@ -486,8 +491,7 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   __shared__ __align__(8) uint64_t bars[3 * kWStages + 5];
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_flag_s;
-  __shared__ RowsOrder ord;
-  __shared__ __align__(16) uint32_t strips[kREpiWarps][kRStripBytes / 4];
+  __shared__ WgradOrder ord;
   volatile int* abort_flag = &abort_flag_s;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -499,7 +503,9 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   const int cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
   const int E = p.E;
 
-  if (warp == 0) load_spans(*reinterpret_cast<RaggedSpans*>(&ord), p.offsets, E, p.R, 256);
+  // (the spans' tiles, which this kernel has no use for, lie where the ring will be)
+  RaggedSpans& spans = *reinterpret_cast<RaggedSpans*>(smem);
+  if (warp == 0) load_spans(spans, p.offsets, E, p.R, 256);
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_u32(&tmem_base_s)), "r"(512u) : "memory");
@@ -520,15 +526,17 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
+  if (threadIdx.x < E + 3) ord.row0[threadIdx.x] = spans.row0[threadIdx.x];
   for (int e = threadIdx.x; e < E; e += kRThreads) {
-    const int mine = ord.row0[e + 2] - ord.row0[e + 1];
+    const int mine = spans.row0[e + 2] - spans.row0[e + 1];
     int rk = 0;
     for (int o = 0; o < E; ++o) {
-      const int other = ord.row0[o + 2] - ord.row0[o + 1];
+      const int other = spans.row0[o + 2] - spans.row0[o + 1];
       rk += (other > mine) || (other == mine && o < e);
     }
     ord.order[rk] = (uint8_t)e;
   }
+  fence_async_proxy();                              // the ring's first loads overwrite the spans
   tcgen05_fence_before();
   __syncthreads();
   cluster_sync_all();
@@ -634,7 +642,7 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     // (the two accumulators have eight warps each: a warp's way from TMEM to memory takes longer than an
     // item's MMAs, and so two of them are under way)
     const int quarter = warp & 3, grp = ((warp - 4) >> 2) & 1, acc = (warp - 4) >> 3;
-    uint8_t* strip = reinterpret_cast<uint8_t*>(strips[warp - 4]);
+    uint8_t* strip = smem + kWStages * kWStageBytes + (warp - 4) * kWStripBytes;
     int turn = 0;
     uint32_t acc_phase = 0;
     for (int item = cluster_id;; item += n_clusters) {
@@ -653,66 +661,55 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       }
       const int prow = w.p0 + 128 * (int)rank + 32 * quarter;     // of lane 0
 #pragma unroll 1
-      for (int part = 0; part < 2; ++part) {
-        const int col = 128 * grp + 64 * part, qcol = w.q0 + col;
-        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + 256 * acc + col;
-        uint32_t o[4][8];
+      for (int part = 0; part < 4; ++part) {
+        const int col = 128 * grp + 32 * part, qcol = w.q0 + col;
+        uint32_t o[16];
         if (!empty) {
-          uint32_t r[4][16];
-#pragma unroll
-          for (int s = 0; s < 4; ++s) tmem_ld16(taddr + 16 * s, r[s]);
+          uint32_t r[2][16];
+          const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + 256 * acc + col;
+          tmem_ld16(taddr, r[0]);
+          tmem_ld16(taddr + 16, r[1]);
           tmem_ld_wait();
 #pragma unroll
-          for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              o[s][i] = two_bf16(__uint_as_float(r[s][2 * i]), __uint_as_float(r[s][2 * i + 1]));
-          if (part == 1) {
+          for (int i = 0; i < 16; ++i)
+            o[i] = two_bf16(__uint_as_float(r[i >> 3][2 * (i & 7)]), __uint_as_float(r[i >> 3][2 * (i & 7) + 1]));
+          if (part == 3) {
             tcgen05_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster((tempty0 + 8 * acc) & kPeerMask);
           }
         } else {
 #pragma unroll
-          for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[s][i] = 0u;
+          for (int i = 0; i < 16; ++i) o[i] = 0u;
         }
-        // through the strip in four passes of eight rows (128 bytes each), 16-byte pieces swizzled by the
-        // row: a store instruction then writes whole 128-byte lines
-        __nv_bfloat16* out = p.out + ((int64_t)w.e * p.P + prow) * p.Q + qcol;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        if (p.wide) {
+          // 32 rows x 64 bytes, 16-byte pieces swizzled as the map says, and off by one TMA store, which
+          // leaves out what lies beyond the expert's matrix
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
-          if ((lane >> 3) == j) {
-            const int rr = lane & 7;
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-              for (int hf = 0; hf < 2; ++hf)
-                *reinterpret_cast<uint4*>(strip + rr * 128 + (((2 * s + hf) ^ rr) << 4)) =
-                    make_uint4(o[s][4 * hf], o[s][4 * hf + 1], o[s][4 * hf + 2], o[s][4 * hf + 3]);
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(strip + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          fence_async_proxy();
+          __syncwarp();
+          if (lane == 0 && prow < p.P && qcol < p.Q) {
+            asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+                         ::"l"(&map_out), "r"(smem_u32(strip)), "r"(qcol), "r"(prow), "r"(w.e) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
-          __syncwarp();
+        } else if (prow + lane < p.P) {
+          __nv_bfloat16* d = p.out + ((int64_t)w.e * p.P + prow + lane) * p.Q + qcol;
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int rr = (lane >> 3) + 4 * k, piece = lane & 7;
-            const uint4 v = *reinterpret_cast<const uint4*>(strip + rr * 128 + ((piece ^ rr) << 4));
-            if (prow + 8 * j + rr >= p.P) continue;
-            __nv_bfloat16* d = out + (int64_t)(8 * j + rr) * p.Q + 8 * piece;
-            const int left = p.Q - qcol - 8 * piece;
-            if (p.wide) {
-              if (left > 0) *reinterpret_cast<uint4*>(d) = v;
-            } else {
-              const __nv_bfloat16* b = reinterpret_cast<const __nv_bfloat16*>(&v);
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (i < left) d[i] = b[i];
-            }
+          for (int i = 0; i < 16; ++i) {
+            const __nv_bfloat162 b = *reinterpret_cast<const __nv_bfloat162*>(&o[i]);
+            if (qcol + 2 * i < p.Q) d[2 * i] = b.x;
+            if (qcol + 2 * i + 1 < p.Q) d[2 * i + 1] = b.y;
           }
         }
       }
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   __syncwarp();
@@ -827,14 +824,20 @@ int ragged_wgrad_tc(const RaggedWgrad& a, cudaStream_t st) {
   MOLE_REQUIRE(p.fault != nullptr, "fault word not allocated");
   p.R = (int)a.R; p.P = a.P; p.Q = a.Q; p.E = a.E;
   p.wide = a.Q % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
-  constexpr size_t smem = (size_t)kWStages * kWStageBytes + 1024;
+  constexpr size_t smem = (size_t)kWStages * kWStageBytes + kREpiWarps * kWStripBytes + 1024;
   static PerDeviceInt cache;
   int pairs = 0;
   if (int rc = resident_pairs(ragged_wgrad_tc_kernel, smem, cache, &pairs)) return rc;
   const int64_t items = (int64_t)a.E * ((a.P + 255) / 256) * ((a.Q + 255) / 256);
   MOLE_REQUIRE(items < (1ll << 31), "%d experts of %d x %d", a.E, a.P, a.Q);
   if (items < pairs) pairs = (int)items;
-  ragged_wgrad_tc_kernel<<<2 * pairs, kRThreads, smem, st>>>(ma, mb, p);
+  CUtensorMap mo = ma;
+  if (p.wide) {
+    const uint64_t dims[3] = {(uint64_t)a.Q, (uint64_t)a.P, (uint64_t)a.E};
+    const uint32_t box_out[3] = {32, 32, 1};
+    if (int rc = encode_map(&mo, a.out, 3, dims, box_out, 2)) return rc;
+  }
+  ragged_wgrad_tc_kernel<<<2 * pairs, kRThreads, smem, st>>>(ma, mb, mo, p);
   MOLE_LAUNCH_OK();
   return MOLE_OK;
 }

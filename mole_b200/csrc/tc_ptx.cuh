@@ -184,9 +184,9 @@ __device__ __forceinline__ void tcgen05_mma2_bf16(uint32_t d_tmem, uint64_t ades
       ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-// Encodes the map of a tensor whose innermost dimension is contiguous: 128-byte swizzle, out-of-range
-// elements read as zeros, dims and box innermost first (box inner extent 128 bytes), elem 2 = bf16, 1 =
-// 8-bit integers.  row_bytes: stride of the second dimension (0: dense), a multiple of 16; the outer
+// Encodes the map of a tensor whose innermost dimension is contiguous: out-of-range elements read as
+// zeros, dims and box innermost first (box inner extent 128 or 64 bytes, swizzled over that span), elem
+// 2 = bf16, 1 = 8-bit integers.  row_bytes: stride of the second dimension (0: dense), a multiple of 16; the outer
 // dimensions are dense on it.
 int encode_map(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint32_t* box, int elem,
                uint64_t row_bytes = 0);
