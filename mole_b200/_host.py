@@ -14,7 +14,8 @@ from . import _lib
 
 _PATH = Path(__file__).resolve().parent / "lib" / "_host.so"
 _ENTRIES = ("mole_grouped_mm", "mole_grouped_mm_workspace_bytes", "mole_grouped_mm_wgrad",
-            "mole_grouped_mm_wgrad_workspace_bytes", "mole_quantize_rows", "mole_grouped_mm_i8", "mole_adam_multi")
+            "mole_grouped_mm_wgrad_workspace_bytes", "mole_quantize_rows", "mole_grouped_mm_i8", "mole_adam_multi",
+            "mole_last_error_string")
 
 
 def _load():

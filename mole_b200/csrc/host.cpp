@@ -11,8 +11,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <stdexcept>
 #include <unordered_set>
 #include <vector>
 
@@ -27,6 +29,7 @@ decltype(&mole_grouped_mm_wgrad_workspace_bytes) grouped_mm_wgrad_workspace_byte
 decltype(&mole_quantize_rows) quantize_rows_;
 decltype(&mole_grouped_mm_i8) grouped_mm_i8_;
 decltype(&mole_adam_multi) adam_multi_;
+decltype(&mole_last_error_string) last_error_string_;
 PyObject* check_ = nullptr;              // raises a non-zero status
 PyObject* out_of_memory_ = nullptr;      // torch.cuda.OutOfMemoryError
 
@@ -50,11 +53,13 @@ void check_with(const at::Tensor& t, const at::Tensor& first) {
   TORCH_CHECK_VALUE(t.device() == first.device(), "tensors are on different devices: ", first.device(), " and ", t.device());
   check_cuda(t);
 }
+// A status that is not zero; where Python has called, `check` turns it into the exception of its kind
+struct StatusError : std::runtime_error {
+  int status;
+  explicit StatusError(int s) : std::runtime_error(last_error_string_()), status(s) {}
+};
 void check_status(int rc) {
-  if (rc == 0) return;
-  PyObject* r = PyObject_CallFunction(check_, "i", rc);
-  Py_XDECREF(r);
-  throw PyRaised();
+  if (rc != 0) throw StatusError(rc);
 }
 bool starts_on_16(const at::Tensor& t) {
   return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.size(-1) * t.element_size() % 16 == 0;
@@ -67,6 +72,10 @@ PyObject* guarded(F&& f) {
   try {
     return f();
   } catch (const PyRaised&) {
+  } catch (const StatusError& e) {
+    PyObject* r = PyObject_CallFunction(check_, "i", e.status);
+    Py_XDECREF(r);
+    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
   } catch (const c10::TypeError& e) {
     PyErr_SetString(PyExc_TypeError, e.what_without_backtrace());
   } catch (const c10::ValueError& e) {
@@ -87,68 +96,104 @@ void check_offsets(const at::Tensor& o, int64_t E) {
 int32_t narrow(int64_t n) {              // sizes that do not fit are refused by the C entry
   return n > INT32_MAX ? INT32_MAX : (int32_t)n;
 }
-at::Tensor output(PyObject* given, const at::Tensor& like, at::IntArrayRef shape, at::ScalarType dtype) {
-  if (given == Py_None) return at::empty(shape, like.options().dtype(dtype));
-  const at::Tensor& out = tensor_of(given, "out");
-  TORCH_CHECK_VALUE(out.sizes() == shape && out.scalar_type() == dtype, "out must be ", dtype, " ", shape);
-  check_with(out, like);
+at::Tensor output(const at::Tensor* given, const at::Tensor& like, at::IntArrayRef shape, at::ScalarType dtype) {
+  if (given == nullptr) return at::empty(shape, like.options().dtype(dtype));
+  TORCH_CHECK_VALUE(given->sizes() == shape && given->scalar_type() == dtype, "out must be ", dtype, " ", shape);
+  check_with(*given, like);
+  return *given;
+}
+const at::Tensor* maybe(PyObject* o) { return o == Py_None ? nullptr : &tensor_of(o, "out"); }
+
+at::Tensor rows_product(const at::Tensor& x, const at::Tensor& w, const at::Tensor& o, bool kn, const at::Tensor* given) {
+  TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 3, "grouped_mm takes x [R, K] and w [E, N, K] or [E, K, N]");
+  const int64_t E = w.size(0), N = w.size(kn ? 2 : 1), K = w.size(kn ? 1 : 2), R = x.size(0);
+  TORCH_CHECK_VALUE(x.size(1) == K, "x has width ", x.size(1), ", the weights take ", K);
+  TORCH_CHECK_TYPE(x.scalar_type() == w.scalar_type(), "x and w must have one dtype");
+  check_offsets(o, E);
+  const int dt = dtype_of(x);
+  check_cuda(x);
+  check_with(w, x);
+  check_with(o, x);
+  c10::cuda::OptionalCUDAGuard guard(x.device());
+  at::Tensor out = output(given, x, {R, N}, x.scalar_type()), ws;
+  int64_t bytes = 0;
+  if (!starts_on_16(x) || !starts_on_16(w)) {
+    check_status(grouped_mm_workspace_bytes_(x.data_ptr(), w.data_ptr(), R, narrow(N), narrow(K), narrow(E), kn,
+                                             (int32_t)x.element_size(), &bytes));
+    ws = bytes_like(x, bytes);
+  }
+  check_status(grouped_mm_(x.data_ptr(), w.data_ptr(), static_cast<const int32_t*>(o.data_ptr()), R, narrow(N), narrow(K),
+                           narrow(E), kn, dt, out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes,
+                           c10::cuda::getCurrentCUDAStream().stream()));
   return out;
 }
+
+at::Tensor weight_gradient(const at::Tensor& a, const at::Tensor& b, const at::Tensor& o, const at::Tensor* given) {
+  TORCH_CHECK_VALUE(a.dim() == 2 && b.dim() == 2 && a.size(0) == b.size(0), "grouped_mm_wgrad takes a [R, P] and b [R, Q]");
+  TORCH_CHECK_TYPE(a.scalar_type() == b.scalar_type(), "a and b must have one dtype");
+  const int64_t E = o.numel() - 1, R = a.size(0), P = a.size(1), Q = b.size(1);
+  check_offsets(o, E);
+  const int dt = dtype_of(a);
+  check_cuda(a);
+  check_with(b, a);
+  check_with(o, a);
+  c10::cuda::OptionalCUDAGuard guard(a.device());
+  at::Tensor out = output(given, a, {E, P, Q}, a.scalar_type()), ws;
+  int64_t bytes = 0;
+  if (!starts_on_16(a) || !starts_on_16(b)) {
+    check_status(grouped_mm_wgrad_workspace_bytes_(a.data_ptr(), b.data_ptr(), R, narrow(P), narrow(Q), narrow(E), dt, &bytes));
+    ws = bytes_like(a, bytes);
+  }
+  check_status(grouped_mm_wgrad_(a.data_ptr(), b.data_ptr(), static_cast<const int32_t*>(o.data_ptr()), R, narrow(P), narrow(Q),
+                                 narrow(E), dt, out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes,
+                                 c10::cuda::getCurrentCUDAStream().stream()));
+  return out;
+}
+
+// The product with its gradients: dx is the same product of dy in the weights' other layout, dw the
+// products of the rows of each expert.
+struct GroupedMM : torch::autograd::Function<GroupedMM> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
+                            const at::Tensor& offsets, bool kn) {
+    ctx->save_for_backward({x, w, offsets});
+    ctx->saved_data["kn"] = kn;
+    return rows_product(x, w, offsets, kn, nullptr);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &w = saved[1], &offsets = saved[2];
+    const bool kn = ctx->saved_data["kn"].toBool();
+    TORCH_CHECK(!(at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || grads[0].requires_grad())),
+                "grouped_mm can be differentiated once only");
+    const at::Tensor dy = grads[0].contiguous();
+    at::Tensor dx, dw;
+    if (ctx->needs_input_grad(0)) dx = rows_product(dy, w, offsets, !kn, nullptr);
+    if (ctx->needs_input_grad(1)) dw = kn ? weight_gradient(x, dy, offsets, nullptr) : weight_gradient(dy, x, offsets, nullptr);
+    return {dx, dw, at::Tensor(), at::Tensor()};
+  }
+};
 
 // grouped_mm(x, w, offsets, w_kn, out)
 PyObject* py_grouped_mm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     TORCH_CHECK(n == 5, "grouped_mm takes 5 arguments");
-    const at::Tensor &x = tensor_of(a[0], "x"), &w = tensor_of(a[1], "w"), &o = tensor_of(a[2], "offsets");
-    const bool kn = PyObject_IsTrue(a[3]) == 1;
-    TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 3, "grouped_mm takes x [R, K] and w [E, N, K] or [E, K, N]");
-    const int64_t E = w.size(0), N = w.size(kn ? 2 : 1), K = w.size(kn ? 1 : 2), R = x.size(0);
-    TORCH_CHECK_VALUE(x.size(1) == K, "x has width ", x.size(1), ", the weights take ", K);
-    TORCH_CHECK_TYPE(x.scalar_type() == w.scalar_type(), "x and w must have one dtype");
-    check_offsets(o, E);
-    const int dt = dtype_of(x);
-    check_cuda(x);
-    check_with(w, x);
-    check_with(o, x);
-    c10::cuda::OptionalCUDAGuard guard(x.device());
-    at::Tensor out = output(a[4], x, {R, N}, x.scalar_type()), ws;
-    int64_t bytes = 0;
-    if (!starts_on_16(x) || !starts_on_16(w)) {
-      check_status(grouped_mm_workspace_bytes_(x.data_ptr(), w.data_ptr(), R, narrow(N), narrow(K), narrow(E), kn,
-                                               (int32_t)x.element_size(), &bytes));
-      ws = bytes_like(x, bytes);
-    }
-    check_status(grouped_mm_(x.data_ptr(), w.data_ptr(), static_cast<const int32_t*>(o.data_ptr()), R, narrow(N), narrow(K),
-                             narrow(E), kn, dt, out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes,
-                             c10::cuda::getCurrentCUDAStream().stream()));
-    return THPVariable_Wrap(out);
+    return THPVariable_Wrap(rows_product(tensor_of(a[0], "x"), tensor_of(a[1], "w"), tensor_of(a[2], "offsets"),
+                                         PyObject_IsTrue(a[3]) == 1, maybe(a[4])));
   });
 }
-
+// grouped_mm_autograd(x, w, offsets, w_kn)
+PyObject* py_grouped_mm_autograd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    TORCH_CHECK(n == 4, "grouped_mm_autograd takes 4 arguments");
+    return THPVariable_Wrap(GroupedMM::apply(tensor_of(a[0], "x"), tensor_of(a[1], "w"), tensor_of(a[2], "offsets"),
+                                             PyObject_IsTrue(a[3]) == 1));
+  });
+}
 // grouped_mm_wgrad(a, b, offsets, out)
-PyObject* py_grouped_mm_wgrad(PyObject*, PyObject* const* v, Py_ssize_t n) {
+PyObject* py_grouped_mm_wgrad(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     TORCH_CHECK(n == 4, "grouped_mm_wgrad takes 4 arguments");
-    const at::Tensor &a = tensor_of(v[0], "a"), &b = tensor_of(v[1], "b"), &o = tensor_of(v[2], "offsets");
-    TORCH_CHECK_VALUE(a.dim() == 2 && b.dim() == 2 && a.size(0) == b.size(0), "grouped_mm_wgrad takes a [R, P] and b [R, Q]");
-    TORCH_CHECK_TYPE(a.scalar_type() == b.scalar_type(), "a and b must have one dtype");
-    const int64_t E = o.numel() - 1, R = a.size(0), P = a.size(1), Q = b.size(1);
-    check_offsets(o, E);
-    const int dt = dtype_of(a);
-    check_cuda(a);
-    check_with(b, a);
-    check_with(o, a);
-    c10::cuda::OptionalCUDAGuard guard(a.device());
-    at::Tensor out = output(v[3], a, {E, P, Q}, a.scalar_type()), ws;
-    int64_t bytes = 0;
-    if (!starts_on_16(a) || !starts_on_16(b)) {
-      check_status(grouped_mm_wgrad_workspace_bytes_(a.data_ptr(), b.data_ptr(), R, narrow(P), narrow(Q), narrow(E), dt, &bytes));
-      ws = bytes_like(a, bytes);
-    }
-    check_status(grouped_mm_wgrad_(a.data_ptr(), b.data_ptr(), static_cast<const int32_t*>(o.data_ptr()), R, narrow(P), narrow(Q),
-                                   narrow(E), dt, out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes,
-                                   c10::cuda::getCurrentCUDAStream().stream()));
-    return THPVariable_Wrap(out);
+    return THPVariable_Wrap(weight_gradient(tensor_of(a[0], "a"), tensor_of(a[1], "b"), tensor_of(a[2], "offsets"), maybe(a[3])));
   });
 }
 
@@ -205,7 +250,7 @@ PyObject* py_mm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check_with(w, q);
     check_with(ws, q);
     c10::cuda::OptionalCUDAGuard guard(q.device());
-    at::Tensor out = output(a[6], q, {R, N}, dtype), scratch;
+    at::Tensor out = output(maybe(a[6]), q, {R, N}, dtype), scratch;
     int64_t bytes = 0;
     if (!starts_on_16(q) || !starts_on_16(w)) {
       check_status(grouped_mm_workspace_bytes_(q.data_ptr(), w.data_ptr(), R, narrow(N), narrow(K), narrow(E), 0, 1, &bytes));
@@ -319,6 +364,7 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   MOLE_BIND(quantize_rows);
   MOLE_BIND(grouped_mm_i8);
   MOLE_BIND(adam_multi);
+  MOLE_BIND(last_error_string);
 #undef MOLE_BIND
   Py_INCREF(a[1]);
   Py_XSETREF(check_, a[1]);
@@ -330,6 +376,7 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define MOLE_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {MOLE_METHOD(bind),          MOLE_METHOD(grouped_mm), MOLE_METHOD(grouped_mm_wgrad),
                          MOLE_METHOD(quantize_rows), MOLE_METHOD(mm_int8),    MOLE_METHOD(adam_multi),
+                         MOLE_METHOD(grouped_mm_autograd),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

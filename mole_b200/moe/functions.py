@@ -7,7 +7,8 @@
   Combine         fast_decode               (layer.py:456-458)   -> [T, M]
   pfetchbwd       backward-prefetch trigger (layer.py:435-436)
 
-  GroupedMM       the expert products alone, over rows packed without capacity or padding
+  grouped_mm      the expert products alone, over rows packed without capacity or padding (its node
+                  is native: csrc/host.cpp)
 
 ``BatchFusedFWD`` and ``pfetchbwd`` are used by the reference layer but defined nowhere in its
 tree; they are written here from their call sites and from ``_MOLECore::forward/backward``
@@ -18,6 +19,7 @@ from __future__ import annotations
 import torch
 
 from .. import ops
+from .._host import host
 from ..utils.Utimer import UATimer
 
 
@@ -195,31 +197,9 @@ class pfetchbwd(torch.autograd.Function):
         return grad, None
 
 
-class GroupedMM(torch.autograd.Function):
-    """``ops.grouped_mm`` with its gradients: dx is the same product of dy in the weights' other layout,
-    dw the products of the rows of each expert."""
-
-    @staticmethod
-    def forward(ctx, x, w, offsets, w_kn):
-        ctx.save_for_backward(x, w, offsets)
-        ctx.w_kn = w_kn
-        return ops.grouped_mm(x, w, offsets, w_kn)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, w, offsets = ctx.saved_tensors
-        dy = dy.contiguous()
-        dx = dw = None
-        if ctx.needs_input_grad[0]:
-            dx = ops.grouped_mm(dy, w, offsets, not ctx.w_kn)
-        if ctx.needs_input_grad[1]:
-            dw = ops.grouped_mm_wgrad(x, dy, offsets) if ctx.w_kn else ops.grouped_mm_wgrad(dy, x, offsets)
-        return dx, dw, None, None
-
-
 def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, w_kn: bool = False) -> torch.Tensor:
     """Differentiable product of rows packed by expert with their expert's weights: ``x[r] @ w[e].T``
     (``w [E, N, K]``) or ``x[r] @ w[e]`` (``w_kn``, ``w [E, K, N]``) for ``offsets[e] <= r < offsets[e + 1]``; rows
-    of no expert come out as zeros and get zero gradients.  See ``ops.grouped_mm``."""
-    return GroupedMM.apply(x, w, offsets, bool(w_kn))
+    of no expert come out as zeros and get zero gradients.  Can be differentiated once.  See
+    ``ops.grouped_mm``."""
+    return host.grouped_mm_autograd(x, w, offsets, w_kn)

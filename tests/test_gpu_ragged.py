@@ -209,6 +209,22 @@ def test_gradients(dtype, k, n, kn):
     close(g1, *want_rows(torch.ones_like(dy), w.detach(), o, not kn), n, "dx of a sum")
 
 
+def test_second_derivatives_are_refused():
+    import mole_b200
+    x, w, o = rnd(10, 16).requires_grad_(), rnd(2, 8, 16, seed=1).requires_grad_(), offs([4, 6])
+    y = mole_b200.grouped_mm(x, w, o)
+    with pytest.raises(RuntimeError, match="once only"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+    y = mole_b200.grouped_mm(x, w, o)
+    with torch.no_grad():
+        w.mul_(2)                                     # what backward needs has been changed
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    assert not mole_b200.grouped_mm(x.detach(), w.detach(), o).requires_grad
+    with torch.no_grad():
+        assert not mole_b200.grouped_mm(x, w, o).requires_grad
+
+
 def test_gradients_against_differences():
     """fp32: the product is bilinear, so a central difference along a direction is its derivative up to
     the rounding of two values: each is off by (K + 2) 2^-24 sum |x w| |dy|, over a step of 2^-3."""
