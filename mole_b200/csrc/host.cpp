@@ -61,9 +61,6 @@ struct StatusError : std::runtime_error {
 void check_status(int rc) {
   if (rc != 0) throw StatusError(rc);
 }
-bool starts_on_16(const at::Tensor& t) {
-  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.size(-1) * t.element_size() % 16 == 0;
-}
 at::Tensor bytes_like(const at::Tensor& t, int64_t n) { return at::empty({n}, t.options().dtype(at::kByte)); }
 
 // No C++ exception passes into the interpreter
@@ -117,11 +114,9 @@ at::Tensor rows_product(const at::Tensor& x, const at::Tensor& w, const at::Tens
   c10::cuda::OptionalCUDAGuard guard(x.device());
   at::Tensor out = output(given, x, {R, N}, x.scalar_type()), ws;
   int64_t bytes = 0;
-  if (!starts_on_16(x) || !starts_on_16(w)) {
-    check_status(grouped_mm_workspace_bytes_(x.data_ptr(), w.data_ptr(), R, narrow(N), narrow(K), narrow(E), kn,
-                                             (int32_t)x.element_size(), &bytes));
-    ws = bytes_like(x, bytes);
-  }
+  check_status(grouped_mm_workspace_bytes_(x.data_ptr(), w.data_ptr(), R, narrow(N), narrow(K), narrow(E), kn,
+                                           (int32_t)x.element_size(), &bytes));
+  if (bytes) ws = bytes_like(x, bytes);
   check_status(grouped_mm_(x.data_ptr(), w.data_ptr(), static_cast<const int32_t*>(o.data_ptr()), R, narrow(N), narrow(K),
                            narrow(E), kn, dt, out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes,
                            c10::cuda::getCurrentCUDAStream().stream()));
@@ -140,10 +135,8 @@ at::Tensor weight_gradient(const at::Tensor& a, const at::Tensor& b, const at::T
   c10::cuda::OptionalCUDAGuard guard(a.device());
   at::Tensor out = output(given, a, {E, P, Q}, a.scalar_type()), ws;
   int64_t bytes = 0;
-  if (!starts_on_16(a) || !starts_on_16(b)) {
-    check_status(grouped_mm_wgrad_workspace_bytes_(a.data_ptr(), b.data_ptr(), R, narrow(P), narrow(Q), narrow(E), dt, &bytes));
-    ws = bytes_like(a, bytes);
-  }
+  check_status(grouped_mm_wgrad_workspace_bytes_(a.data_ptr(), b.data_ptr(), R, narrow(P), narrow(Q), narrow(E), dt, &bytes));
+  if (bytes) ws = bytes_like(a, bytes);
   check_status(grouped_mm_wgrad_(a.data_ptr(), b.data_ptr(), static_cast<const int32_t*>(o.data_ptr()), R, narrow(P), narrow(Q),
                                  narrow(E), dt, out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes,
                                  c10::cuda::getCurrentCUDAStream().stream()));
@@ -252,10 +245,8 @@ PyObject* py_mm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     c10::cuda::OptionalCUDAGuard guard(q.device());
     at::Tensor out = output(maybe(a[6]), q, {R, N}, dtype), scratch;
     int64_t bytes = 0;
-    if (!starts_on_16(q) || !starts_on_16(w)) {
-      check_status(grouped_mm_workspace_bytes_(q.data_ptr(), w.data_ptr(), R, narrow(N), narrow(K), narrow(E), 0, 1, &bytes));
-      scratch = bytes_like(q, bytes);
-    }
+    check_status(grouped_mm_workspace_bytes_(q.data_ptr(), w.data_ptr(), R, narrow(N), narrow(K), narrow(E), 0, 1, &bytes));
+    if (bytes) scratch = bytes_like(q, bytes);
     check_status(grouped_mm_i8_(q.data_ptr(), static_cast<const float*>(qs.data_ptr()), w.data_ptr(),
                                 static_cast<const float*>(ws.data_ptr()), offsets, R, narrow(N), narrow(K), narrow(E),
                                 dtype == at::kFloat ? MOLE_F32 : MOLE_BF16, out.data_ptr(),

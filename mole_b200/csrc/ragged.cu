@@ -140,29 +140,55 @@ static int launch_quantize(const void* x, int64_t R, int K, void* q, float* scal
   return MOLE_OK;
 }
 
-// ---- operands that the tensor cores cannot address ------------------------------------------------
+// ---- operands that the tensor cores cannot address, partial results ------------------------------------------------
 // TMA wants rows that start on 16 bytes.  Operands of other widths or at other addresses are copied to
 // rows that do, in the caller's workspace; the copy costs a pass of HBM over the operand (weights:
 // only those of experts that have rows), the products on the CUDA cores an order of magnitude.
-// A thread stores 16 bytes; matrix m of `rows` rows belongs to expert m, one matrix belongs to all.
-template <typename T>
+// A thread makes 16 bytes of the copy from two aligned pieces; matrix m of `rows` rows belongs to expert m, one matrix belongs to all.
 __global__ void __launch_bounds__(256)
-align_rows_kernel(const T* __restrict__ src, int64_t rows, int cols, int ld, T* __restrict__ dst,
+align_rows_kernel(const uint8_t* __restrict__ src, int64_t rows, int row_bytes, int ld_bytes, uint8_t* __restrict__ dst,
                   const int32_t* __restrict__ offsets) {
-  constexpr int V = 16 / sizeof(T);
   if (offsets != nullptr && offsets[blockIdx.y + 1] <= offsets[blockIdx.y]) return;
-  const int per_row = ld / V;
+  const int per_row = ld_bytes / 16;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows * per_row) return;
   const int64_t r = i / per_row;
-  const int c = (int)(i - r * per_row) * V;
-  const T* s = src + ((int64_t)blockIdx.y * rows + r) * cols + c;
-  T v[V];
+  const int c = (int)(i - r * per_row) * 16;
+  const int64_t matrix = rows * row_bytes;
+  const uint8_t* first = src, *last = src + (int64_t)gridDim.y * matrix;         // what may be read
+  const uint8_t* s = src + (int64_t)blockIdx.y * matrix + r * row_bytes + c;
+  const uint8_t* at = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(s) & ~static_cast<uintptr_t>(15));
+  uint32_t o[4];
+  if (at >= first && at + 32 <= last) {
+    // the two aligned pieces that hold the sixteen bytes, moved down by the distance in words and bytes
+    const uint4 a = *reinterpret_cast<const uint4*>(at), b = *reinterpret_cast<const uint4*>(at + 16);
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    const int off = (int)(s - at);
+    if (off & 8) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) v[j] = c + j < cols ? s[j] : T(0);
-  uint4 o;
-  memcpy(&o, v, 16);
-  *reinterpret_cast<uint4*>(dst + ((int64_t)blockIdx.y * rows + r) * ld + c) = o;
+      for (int j = 0; j < 6; ++j) w[j] = w[j + 2];
+    }
+    if (off & 4) {
+#pragma unroll
+      for (int j = 0; j < 5; ++j) w[j] = w[j + 1];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = __funnelshift_r(w[j], w[j + 1], 8 * (off & 3));
+    const int left = row_bytes - c;                  // bytes behind the row's end are zeros
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = left - 4 * j;
+      if (n < 4) o[j] = n > 0 ? o[j] & ((1u << (8 * n)) - 1u) : 0u;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      o[j] = 0;
+      for (int k = 0; k < 4; ++k)
+        if (c + 4 * j + k < row_bytes) o[j] |= (uint32_t)s[4 * j + k] << (8 * k);
+    }
+  }
+  *reinterpret_cast<uint4*>(dst + ((int64_t)blockIdx.y * rows + r) * ld_bytes + c) = make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 static bool aligned_to(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -185,14 +211,21 @@ static int align_operand(Aligner& ws, const void** p, int64_t matrices, int64_t 
                "workspace of %lld bytes, %lld needed (mole_grouped_mm_workspace_bytes)", (long long)ws.left, (long long)ws.used);
   void* dst = ws.at + ws.used - bytes;
   const dim3 grid((unsigned)((rows * (*ld / unit) + 255) / 256), (unsigned)matrices);
-  if (elem == 1)
-    align_rows_kernel<int8_t><<<grid, 256, 0, st>>>(static_cast<const int8_t*>(*p), rows, cols, *ld,
-                                                    static_cast<int8_t*>(dst), offsets);
-  else
-    align_rows_kernel<uint16_t><<<grid, 256, 0, st>>>(static_cast<const uint16_t*>(*p), rows, cols, *ld,
-                                                      static_cast<uint16_t*>(dst), offsets);
+  align_rows_kernel<<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(*p), rows, cols * elem, *ld * elem,
+                                          static_cast<uint8_t*>(dst), offsets);
   MOLE_LAUNCH_OK();
   *p = dst;
+  return MOLE_OK;
+}
+// room for the partial results of a cut reduction
+static int take_parts(Aligner& ws, int split, int64_t n, float** part) {
+  if (split <= 1) return MOLE_OK;
+  const int64_t bytes = ((int64_t)split * n * 4 + 255) / 256 * 256;
+  ws.used += bytes;
+  if (ws.count_only) return MOLE_OK;
+  MOLE_REQUIRE(ws.at != nullptr && ws.used <= ws.left && aligned_to(ws.at, 16),
+               "workspace of %lld bytes, %lld needed (mole_grouped_mm_workspace_bytes)", (long long)ws.left, (long long)ws.used);
+  *part = reinterpret_cast<float*>(ws.at + ws.used - bytes);
   return MOLE_OK;
 }
 static int align_rows(RaggedRows& a, int elem, Aligner ws, int64_t* used, cudaStream_t st) {
@@ -227,8 +260,13 @@ extern "C" int mole_grouped_mm(const void* x, const void* w, const int32_t* offs
   a.R = R; a.N = N; a.K = K; a.E = E; a.kn = w_kn != 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (ragged_rows_few_takes(a)) return ragged_rows_few(dtype, a, st);
-  if (dtype == MOLE_F32) return ragged_rows_simt(a, st);
-  if (int rc = align_rows(a, 2, Aligner{static_cast<uint8_t*>(workspace), workspace_bytes, 0, false}, nullptr, st)) return rc;
+  Aligner ws{static_cast<uint8_t*>(workspace), workspace_bytes, 0, false};
+  if (dtype == MOLE_F32) {
+    a.split = ragged_rows_simt_split(a);
+    if (int rc = take_parts(ws, a.split, R * N, &a.part)) return rc;
+    return ragged_rows_simt(a, st);
+  }
+  if (int rc = align_rows(a, 2, ws, nullptr, st)) return rc;
   return ragged_rows_tc(2, dtype, a, st);
 }
 
@@ -240,7 +278,13 @@ extern "C" int mole_grouped_mm_workspace_bytes(const void* x, const void* w, int
   a.x = x; a.w = w;
   a.R = R; a.N = N; a.K = K; a.E = E; a.kn = w_kn != 0;
   *bytes = 0;
-  if (elem_bytes == 4 || ragged_rows_few_takes(a)) return MOLE_OK;
+  if (R == 0 || ragged_rows_few_takes(a)) return MOLE_OK;
+  if (elem_bytes == 4) {
+    Aligner ws{nullptr, 0, 0, true};
+    if (int rc = take_parts(ws, ragged_rows_simt_split(a), R * N, nullptr)) return rc;
+    *bytes = ws.used;
+    return MOLE_OK;
+  }
   return align_rows(a, elem_bytes, Aligner{nullptr, 0, 0, true}, bytes, nullptr);
 }
 
@@ -257,12 +301,14 @@ extern "C" int mole_grouped_mm_wgrad(const void* a, const void* b, const int32_t
   g.a = a; g.b = b; g.offsets = offsets; g.out = out;
   g.R = R; g.P = P; g.Q = Q; g.E = E;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Aligner ws{static_cast<uint8_t*>(workspace), workspace_bytes, 0, false};
+  g.split = ragged_wgrad_split(dtype == MOLE_BF16, g);
+  if (int rc = take_parts(ws, g.split, (int64_t)E * P * Q, &g.part)) return rc;
   if (dtype == MOLE_F32) return ragged_wgrad_simt(g, st);
   if (R == 0) {
     MOLE_CUDA_OK(cudaMemsetAsync(out, 0, (size_t)E * P * Q * size, st));
     return MOLE_OK;
   }
-  Aligner ws{static_cast<uint8_t*>(workspace), workspace_bytes, 0, false};
   if (int rc = align_operand(ws, &g.a, 1, R, P, 2, &g.lda, nullptr, st)) return rc;
   if (int rc = align_operand(ws, &g.b, 1, R, Q, 2, &g.ldb, nullptr, st)) return rc;
   return ragged_wgrad_tc(g, st);
@@ -273,9 +319,14 @@ extern "C" int mole_grouped_mm_wgrad_workspace_bytes(const void* a, const void* 
   if (int rc = check_sizes(R, P, Q, E)) return rc;
   MOLE_REQUIRE(bytes != nullptr && (dtype == MOLE_F32 || dtype == MOLE_BF16), "bad argument");
   *bytes = 0;
-  if (dtype == MOLE_F32 || R == 0) return MOLE_OK;
+  if (R == 0) return MOLE_OK;
   Aligner ws{nullptr, 0, 0, true};
   int ld = 0;
+  RaggedWgrad g{};
+  g.R = R; g.P = P; g.Q = Q; g.E = E;
+  if (int rc = take_parts(ws, ragged_wgrad_split(dtype == MOLE_BF16, g), (int64_t)E * P * Q, nullptr)) return rc;
+  *bytes = ws.used;
+  if (dtype == MOLE_F32) return MOLE_OK;
   if (int rc = align_operand(ws, &a, 1, R, P, 2, &ld, nullptr, nullptr)) return rc;
   if (int rc = align_operand(ws, &b, 1, R, Q, 2, &ld, nullptr, nullptr)) return rc;
   *bytes = ws.used;

@@ -19,6 +19,8 @@ struct RaggedRows {         // out[r, n] = sum_k x[r, k] w_e(n, k)
   int64_t R;
   int N, K, E, kn;
   int ldx, ldw;             // elements between rows of x, and of w's inner matrices
+  float* part;              // fp32: room for `split` partial results [R, N] (split > 1)
+  int split;
 };
 struct RaggedWgrad {        // out[e, p, q] = sum over the rows r of e of a[r, p] b[r, q]
   const void* a;            // [R, P]
@@ -28,10 +30,17 @@ struct RaggedWgrad {        // out[e, p, q] = sum over the rows r of e of a[r, p
   int64_t R;
   int P, Q, E;
   int lda, ldb;
+  float* part;              // room for `split` partial results [E, P, Q] (split > 1)
+  int split;
 };
 
 int ragged_rows_simt(const RaggedRows& a, cudaStream_t st);          // fp32
 int ragged_wgrad_simt(const RaggedWgrad& a, cudaStream_t st);
+// Into how many parts the reduction is cut where there are too few tiles for the SMs; partial results
+// are added in their order by ragged_join.
+int ragged_rows_simt_split(const RaggedRows& a);
+int ragged_wgrad_split(bool tensor, const RaggedWgrad& a);
+int ragged_join(int out_dtype, const float* part, int split, int64_t n, void* out, cudaStream_t st);
 // up to 16 rows, every type (ldx = K, ldw dense)
 bool ragged_rows_few_takes(const RaggedRows& a);
 int ragged_rows_few(int dtype, const RaggedRows& a, cudaStream_t st);

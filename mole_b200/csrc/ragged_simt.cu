@@ -4,8 +4,9 @@
 // A thread block takes a tile of T x T outputs, a thread (T / 16)^2 of them in registers; tiles of both
 // operands, 16 deep in the reduction, go through shared memory, the next ones on their way in
 // registers meanwhile.  With T = 128 a thread makes 64 multiply-adds per step on four 16-byte reads.
-// T = 64 where experts have few rows.  Sums run over the reduction in its order, one fused
-// multiply-add after the other.  Bound by the fp32 pipes: 8192 rows, 8 experts of 512 x 2048 in 0.45 ms
+// T = 64 where experts have few rows, and 16 rows for a tile that holds no more.  Sums run over the
+// reduction in its order, one fused multiply-add after the other; where there are too few tiles for
+// the SMs the reduction is cut into parts, joined in their order by a second kernel.  Bound by the fp32 pipes: 8192 rows, 8 experts of 512 x 2048 in 0.45 ms
 // each way, 38 to 41 TFLOP/s, which is what a plain loop of library products reaches; pairs on the
 // packed instructions (0.52 ms), fragments read one step ahead and one block of twice the registers
 // per SM (0.45 to 0.5) are no faster.
@@ -101,6 +102,78 @@ __device__ __forceinline__ void tile_product(const float* pa, int64_t lda, int m
   }
 }
 
+// The same for a tile of at most 16 rows and 64 columns: four groups of 64 threads take a quarter of every
+// 64 elements of the reduction each (so that nothing is multiplied for rows that are not there) and
+// are added in their order.
+template <bool A_K, bool B_K, bool WIDE>
+__device__ __forceinline__ void few_rows_product(const float* pa, int64_t lda, int m_left, const float* pb, int64_t ldb,
+                                                 int n_left, int K, float (&acc)[4][4]) {
+  constexpr int D = 64;
+  __shared__ __align__(16) float as[D][16 + 4], bs[D][64 + 4];
+  const int t = threadIdx.x, g = t >> 6, ty = (t >> 4) & 3, tx = t & 15;
+  static_assert(A_K, "rows are read along the reduction");
+  for (int k0 = 0; k0 < K; k0 += D) {
+    __syncthreads();
+    {
+      const int m = t >> 4, k = (t & 15) * 4;                     // 16 rows x 64, four each
+#pragma unroll
+      for (int i = 0; i < 4; ++i) as[k + i][m] = m < m_left && k0 + k + i < K ? pa[(int64_t)m * lda + k0 + k + i] : 0.f;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {                                 // 64 x 64, twice eight each
+      float v[8];
+      if (B_K) {
+        const int n = t & 63, k = (t >> 6) * 8 + 32 * h;
+        load8<WIDE>(pb + (int64_t)n * ldb + k0 + k, n < n_left ? K - k0 - k : 0, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) bs[k + i][n] = v[i];
+      } else {
+        const int k = (t >> 3) + 32 * h, n = (t & 7) * 8;
+        load8<WIDE>(pb + (int64_t)(k0 + k) * ldb + n, k0 + k < K ? n_left - n : 0, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) bs[k][n + i] = v[i];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      float x[4], y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { x[i] = as[16 * g + k][4 * ty + i]; y[i] = bs[16 * g + k][4 * tx + i]; }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
+    }
+  }
+  __syncthreads();
+  float (*sums)[16][64 + 4] = reinterpret_cast<float (*)[16][64 + 4]>(&bs[0][0]);       // [4], as large as bs
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[g][4 * ty + i][4 * tx + j] = acc[i][j];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      acc[i][j] = 0.f;
+      if (g == 0)
+        for (int q = 0; q < 4; ++q) acc[i][j] += sums[q][4 * ty + i][4 * tx + j];
+    }
+}
+
+// Four neighbouring columns of a row; `left` of them exist.  `vec`: rows of out start on 16 bytes.
+__device__ __forceinline__ void put4(float* d, const float* v, int left, bool vec) {
+  if (vec && left >= 4) {
+    *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) d[j] = v[j];
+  }
+}
+
 template <int T, bool KN, bool WIDE>
 __global__ void __launch_bounds__(256, T == 128 ? 2 : 4)
 ragged_rows_kernel(const RaggedRows a) {
@@ -113,15 +186,32 @@ ragged_rows_kernel(const RaggedRows a) {
   const int span = span_of(sp, a.E, tile);
   const int r0 = sp.row0[span] + (tile - sp.tile0[span]) * T, rend = sp.row0[span + 1];
   const int n0 = blockIdx.y * T;
-  float* out = static_cast<float*>(a.out);
+  // part z of the reduction
+  const int share = (a.K + a.split * kSK - 1) / (a.split * kSK) * kSK;
+  const int k0 = blockIdx.z * share, len = min(a.K - k0, share);          // len <= 0: nothing left for this part
+  float* out = a.split > 1 ? a.part + (int64_t)blockIdx.z * a.R * a.N : static_cast<float*>(a.out);
+  const bool vec = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   const int e = span - 1;
   const bool owned = e >= 0 && e < a.E;
   float acc[M][M] = {};
   if (owned) {
-    const float* x = static_cast<const float*>(a.x) + (int64_t)r0 * a.K;
-    const float* w = static_cast<const float*>(a.w) + (int64_t)e * a.N * a.K;
-    tile_product<T, true, !KN, WIDE>(x, a.K, rend - r0, KN ? w + n0 : w + (int64_t)n0 * a.K, KN ? a.N : a.K, a.N - n0,
-                                         a.K, acc);
+    const float* x = static_cast<const float*>(a.x) + (int64_t)r0 * a.K + k0;
+    const float* w = static_cast<const float*>(a.w) + (int64_t)e * a.N * a.K + (KN ? (int64_t)k0 * a.N : (int64_t)k0);
+    const float* wt = KN ? w + n0 : w + (int64_t)n0 * a.K;
+    const int64_t ldw = KN ? a.N : a.K;
+    if constexpr (T == 64) {
+      if (rend - r0 <= 16) {
+        few_rows_product<true, !KN, WIDE>(x, a.K, rend - r0, wt, ldw, a.N - n0, len, acc);
+        const int t = threadIdx.x, ty = (t >> 4) & 3, tx = t & 15;
+        if (t < 64)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (r0 + 4 * ty + i < rend)
+              put4(out + (int64_t)(r0 + 4 * ty + i) * a.N + n0 + 4 * tx, acc[i], a.N - n0 - 4 * tx, vec);
+        return;
+      }
+    }
+    if (len > 0) tile_product<T, true, !KN, WIDE>(x, a.K, rend - r0, wt, ldw, a.N - n0, len, acc);
   }
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
 #pragma unroll
@@ -129,10 +219,22 @@ ragged_rows_kernel(const RaggedRows a) {
     const int r = r0 + tile_index<T>(ty, i);
     if (r >= rend) continue;
 #pragma unroll
-    for (int j = 0; j < M; ++j) {
+    for (int j = 0; j < M; j += 4) {
       const int n = n0 + tile_index<T>(tx, j);
-      if (n < a.N) out[(int64_t)r * a.N + n] = acc[i][j];
+      put4(out + (int64_t)r * a.N + n, &acc[i][j], a.N - n, vec);
     }
+  }
+}
+
+// Rows of one expert, by a whole block: the running maximum over the offsets before it only where they do
+// not rise by themselves
+__device__ __forceinline__ void expert_rows(const int32_t* offsets, int E, int R, int e, int& first, int& end) {
+  auto at = [&](int i) { return min(max(offsets[i], 0), R); };
+  first = at(e);
+  end = at(e + 1);
+  if (__syncthreads_or(threadIdx.x < E && offsets[threadIdx.x + 1] < offsets[threadIdx.x])) {
+    for (int i = 0; i < e; ++i) first = max(first, at(i));
+    end = max(first, end);
   }
 }
 
@@ -140,36 +242,87 @@ template <int T, bool WIDE>
 __global__ void __launch_bounds__(256, T == 128 ? 2 : 4)
 ragged_wgrad_kernel(const RaggedWgrad a) {
   constexpr int M = T / 16;
-  __shared__ RaggedSpans sp;
-  if (threadIdx.x < 32) load_spans(sp, a.offsets, a.E, (int)a.R, T);
-  __syncthreads();
-  const int e = blockIdx.z, q0 = blockIdx.x * T, p0 = blockIdx.y * T;
-  const int r0 = sp.row0[e + 1], rows = sp.row0[e + 2] - r0;
+  const int e = blockIdx.z / a.split, part = blockIdx.z % a.split, q0 = blockIdx.x * T, p0 = blockIdx.y * T;
+  int first, end;
+  expert_rows(a.offsets, a.E, (int)a.R, e, first, end);
+  const int all = end - first;
+  const int share = (all + a.split * kSK - 1) / (a.split * kSK) * kSK;    // of an expert's rows per part
+  const int r0 = first + part * share, rows = min(share, all - part * share);
   float acc[M][M] = {};
   if (rows > 0)
     tile_product<T, false, false, WIDE>(static_cast<const float*>(a.a) + (int64_t)r0 * a.P + p0, a.P, a.P - p0,
                                             static_cast<const float*>(a.b) + (int64_t)r0 * a.Q + q0, a.Q, a.Q - q0, rows, acc);
-  float* out = static_cast<float*>(a.out) + (int64_t)e * a.P * a.Q;
+  float* out = (a.split > 1 ? a.part + (int64_t)part * a.E * a.P * a.Q : static_cast<float*>(a.out)) + (int64_t)e * a.P * a.Q;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  const bool vec = a.Q % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
 #pragma unroll
   for (int i = 0; i < M; ++i)
 #pragma unroll
-    for (int j = 0; j < M; ++j) {
+    for (int j = 0; j < M; j += 4) {
       const int p = p0 + tile_index<T>(ty, i), q = q0 + tile_index<T>(tx, j);
-      if (p < a.P && q < a.Q) out[(int64_t)p * a.Q + q] = acc[i][j];
+      if (p < a.P) put4(out + (int64_t)p * a.Q + q, &acc[i][j], a.Q - q, vec);
     }
 }
 
 // rows that start on 16 bytes
 static bool wide_rows(const void* p, int64_t ld) { return ld % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// 128-row tiles once experts have about as many rows on average: half a tile per expert is idle
+static int rows_tile(const RaggedRows& a) { return a.R >= 128ll * a.E && a.N > 64 ? 128 : 64; }
+// Into how many parts to cut the reduction: the number that costs least, by this account.  `slots` tiles run
+// at a time, and together they do `rate` operations a second, so cutting pays where the tiles fill the
+// last round (or the only one) badly; partial results are written and read once, at 5 TB/s.
+static int parts_for(int64_t tiles, int tile, int64_t reduction, int64_t outputs, int slots, double rate) {
+  if (tiles < 1) return 1;
+  const double whole = 2.0 * tile * tile * (double)reduction / (rate / slots);        // one tile's time
+  int best = 1;
+  double least = (double)((tiles + slots - 1) / slots) * whole;
+  for (int s = 2; s <= 32 && reduction / s >= 128; ++s) {
+    const double t = (double)((tiles * s + slots - 1) / slots) * whole / s + s * (double)outputs * 8 / 5e12 + 3e-6;
+    if (t < 0.95 * least) { least = t; best = s; }
+  }
+  return best;
+}
+int ragged_rows_simt_split(const RaggedRows& a) {
+  const int T = rows_tile(a);
+  const int64_t live = a.E < a.R ? a.E : a.R;
+  const int64_t tiles = (a.R / T + (live + 1) / 2) * ((a.N + T - 1) / T);     // (half of the experts end in a tile of their own)
+  return parts_for(tiles, T, a.K, a.R * a.N, sm_count() * (T == 128 ? 2 : 4), 4e13);
+}
+static int64_t wgrad_tiles(const RaggedWgrad& a, int T) {
+  return (int64_t)a.E * ((a.P + T - 1) / T) * ((a.Q + T - 1) / T);
+}
+static int wgrad_tile(const RaggedWgrad& a) { return wgrad_tiles(a, 128) >= sm_count() ? 128 : 64; }
+int ragged_wgrad_split(bool tensor, const RaggedWgrad& a) {
+  const int T = tensor ? 256 : wgrad_tile(a);          // on the tensor cores a pair of SMs per tile
+  const int slots = tensor ? sm_count() / 2 : sm_count() * (T == 128 ? 2 : 4);
+  return parts_for(wgrad_tiles(a, T), T, a.R / a.E, (int64_t)a.E * a.P * a.Q, slots, tensor ? 1e15 : 4e13);
+}
+
+// out[i] = part[0][i] + part[1][i] + ...
+template <typename TO>
+__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, int split, int64_t n, TO* __restrict__ out) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float v = part[i];
+    for (int s = 1; s < split; ++s) v += part[(int64_t)s * n + i];
+    out[i] = Elem<TO>::from_f(v);
+  }
+}
+int ragged_join(int out_dtype, const float* part, int split, int64_t n, void* out, cudaStream_t st) {
+  int64_t blocks = (n + 255) / 256;
+  if (blocks > (int64_t)sm_count() * 8) blocks = (int64_t)sm_count() * 8;
+  if (out_dtype == MOLE_F32) join_kernel<<<(unsigned)blocks, 256, 0, st>>>(part, split, n, static_cast<float*>(out));
+  else join_kernel<<<(unsigned)blocks, 256, 0, st>>>(part, split, n, static_cast<__nv_bfloat16*>(out));
+  MOLE_LAUNCH_OK();
+  return MOLE_OK;
+}
+
 template <bool KN>
 static int launch_rows(const RaggedRows& a, cudaStream_t st) {
   const bool wide = wide_rows(a.x, a.K) && wide_rows(a.w, KN ? a.N : a.K);
-  // 128-row tiles once experts have about as many rows on average: half a tile per expert is idle
-  const bool large = a.R >= 128ll * a.E && a.N > 64;
-  auto grid = [&](int T) {
-    return dim3((unsigned)(a.R / T + a.E + 2), (unsigned)((a.N + T - 1) / T));     // every span may end in a partial tile
+  const bool large = rows_tile(a) == 128;
+  auto grid = [&](int T) {                                                   // every span may end in a partial tile
+    return dim3((unsigned)(a.R / T + a.E + 2), (unsigned)((a.N + T - 1) / T), (unsigned)a.split);
   };
   if (large && wide) ragged_rows_kernel<128, KN, true><<<grid(128), 256, 0, st>>>(a);
   else if (large) ragged_rows_kernel<128, KN, false><<<grid(128), 256, 0, st>>>(a);
@@ -180,20 +333,20 @@ static int launch_rows(const RaggedRows& a, cudaStream_t st) {
 }
 
 int ragged_rows_simt(const RaggedRows& a, cudaStream_t st) {
-  return a.kn ? launch_rows<true>(a, st) : launch_rows<false>(a, st);
+  if (int rc = a.kn ? launch_rows<true>(a, st) : launch_rows<false>(a, st)) return rc;
+  return a.split > 1 ? ragged_join(MOLE_F32, a.part, a.split, a.R * a.N, a.out, st) : MOLE_OK;
 }
 int ragged_wgrad_simt(const RaggedWgrad& a, cudaStream_t st) {
   const bool wide = wide_rows(a.a, a.P) && wide_rows(a.b, a.Q);
-  // 128 x 128 tiles where they fill the SMs
-  auto grid = [&](int T) { return dim3((unsigned)((a.Q + T - 1) / T), (unsigned)((a.P + T - 1) / T), (unsigned)a.E); };
+  auto grid = [&](int T) { return dim3((unsigned)((a.Q + T - 1) / T), (unsigned)((a.P + T - 1) / T), (unsigned)(a.E * a.split)); };
   const dim3 g = grid(128);
-  const bool large = (int64_t)g.x * g.y * g.z >= 2 * sm_count();
+  const bool large = wgrad_tile(a) == 128;
   if (large && wide) ragged_wgrad_kernel<128, true><<<g, 256, 0, st>>>(a);
   else if (large) ragged_wgrad_kernel<128, false><<<g, 256, 0, st>>>(a);
   else if (wide) ragged_wgrad_kernel<64, true><<<grid(64), 256, 0, st>>>(a);
   else ragged_wgrad_kernel<64, false><<<grid(64), 256, 0, st>>>(a);
   MOLE_LAUNCH_OK();
-  return MOLE_OK;
+  return a.split > 1 ? ragged_join(MOLE_F32, a.part, a.split, (int64_t)a.E * a.P * a.Q, a.out, st) : MOLE_OK;
 }
 
 }  // namespace mole

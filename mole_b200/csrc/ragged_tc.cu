@@ -459,25 +459,33 @@ struct WgradParams {
   int32_t* fault;
   int R, P, Q, E;
   int wide;             // rows of out are multiples of 16 bytes, its base too
+  int split;            // an expert's rows are cut into so many parts,
+  float* part;          // with a result [E, P, Q] each (split > 1)
 };
 struct WgradOrder {
   int row0[kMaxRaggedExperts + 3];
   uint8_t order[kMaxRaggedExperts];      // experts by falling row counts
 };
 struct WgradItem {
-  int valid, e, p0, q0, row0, rows;
+  int valid, e, p0, q0, row0, rows, part;
 };
 __device__ __forceinline__ WgradItem wgrad_item(const WgradOrder& o, const WgradParams& p, int item) {
   WgradItem w;
-  const int qb = (p.Q + 255) / 256, per = (p.P + 255) / 256 * qb;
+  const int qb = (p.Q + 255) / 256, per = (p.P + 255) / 256 * qb * p.split;
   w.valid = item < p.E * per;
   if (!w.valid) return w;
   const int i = item / per, r = item - i * per;
   w.e = o.order[i];
-  w.p0 = r / qb * 256;
-  w.q0 = r % qb * 256;
+  w.part = r % p.split;
+  w.p0 = r / p.split / qb * 256;
+  w.q0 = r / p.split % qb * 256;
   w.row0 = o.row0[w.e + 1];
   w.rows = o.row0[w.e + 2] - w.row0;
+  if (p.split > 1) {
+    const int share = (w.rows + p.split * 64 - 1) / (p.split * 64) * 64;
+    w.row0 += w.part * share;
+    w.rows = max(0, min(share, w.rows - w.part * share));
+  }
   return w;
 }
 
@@ -664,8 +672,8 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       for (int part = 0; part < 4; ++part) {
         const int col = 128 * grp + 32 * part, qcol = w.q0 + col;
         uint32_t o[16];
+        uint32_t r[2][16];
         if (!empty) {
-          uint32_t r[2][16];
           const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + 256 * acc + col;
           tmem_ld16(taddr, r[0]);
           tmem_ld16(taddr + 16, r[1]);
@@ -680,9 +688,24 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = 0u;
+          for (int i = 0; i < 16; ++i) r[0][i] = r[1][i] = o[i] = 0u;
         }
-        if (p.wide) {
+        if (p.split > 1) {
+          if (prow + lane < p.P) {
+            float* d = p.part + (((int64_t)w.part * p.E + w.e) * p.P + prow + lane) * p.Q + qcol;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const uint32_t* v = &r[i >> 4][i & 15];
+              if (p.Q % 4 == 0) {                   // (the parts start on 256 bytes)
+                if (qcol + i < p.Q) *reinterpret_cast<uint4*>(d + i) = make_uint4(v[0], v[1], v[2], v[3]);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  if (qcol + i + j < p.Q) d[i + j] = __uint_as_float(v[j]);
+              }
+            }
+          }
+        } else if (p.wide) {
           // 32 rows x 64 bytes, 16-byte pieces swizzled as the map says, and off by one TMA store, which
           // leaves out what lies beyond the expert's matrix
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -698,13 +721,20 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
                          ::"l"(&map_out), "r"(smem_u32(strip)), "r"(qcol), "r"(prow), "r"(w.e) : "memory");
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
-        } else if (prow + lane < p.P) {
-          __nv_bfloat16* d = p.out + ((int64_t)w.e * p.P + prow + lane) * p.Q + qcol;
+        } else {
+          // rows of the gradient at any address: turned round in the strip, so that a store instruction
+          // writes 32 neighbouring columns of one row
+          __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const __nv_bfloat162 b = *reinterpret_cast<const __nv_bfloat162*>(&o[i]);
-            if (qcol + 2 * i < p.Q) d[2 * i] = b.x;
-            if (qcol + 2 * i + 1 < p.Q) d[2 * i + 1] = b.y;
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(strip + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          __syncwarp();
+          if (qcol + lane < p.Q) {
+            __nv_bfloat16* d = p.out + ((int64_t)w.e * p.P + prow) * p.Q + qcol + lane;
+            for (int i = 0; i < 32 && prow + i < p.P; ++i)
+              d[(int64_t)i * p.Q] = *reinterpret_cast<const __nv_bfloat16*>(
+                  strip + i * 64 + (((lane >> 3) ^ ((i >> 1) & 3)) << 4) + 2 * (lane & 7));
           }
         }
       }
@@ -828,7 +858,9 @@ int ragged_wgrad_tc(const RaggedWgrad& a, cudaStream_t st) {
   static PerDeviceInt cache;
   int pairs = 0;
   if (int rc = resident_pairs(ragged_wgrad_tc_kernel, smem, cache, &pairs)) return rc;
-  const int64_t items = (int64_t)a.E * ((a.P + 255) / 256) * ((a.Q + 255) / 256);
+  p.split = a.split;
+  p.part = a.part;
+  const int64_t items = (int64_t)a.E * a.split * ((a.P + 255) / 256) * ((a.Q + 255) / 256);
   MOLE_REQUIRE(items < (1ll << 31), "%d experts of %d x %d", a.E, a.P, a.Q);
   if (items < pairs) pairs = (int)items;
   CUtensorMap mo = ma;
@@ -839,7 +871,7 @@ int ragged_wgrad_tc(const RaggedWgrad& a, cudaStream_t st) {
   }
   ragged_wgrad_tc_kernel<<<2 * pairs, kRThreads, smem, st>>>(ma, mb, mo, p);
   MOLE_LAUNCH_OK();
-  return MOLE_OK;
+  return a.split > 1 ? ragged_join(MOLE_BF16, a.part, a.split, (int64_t)a.E * a.P * a.Q, a.out, st) : MOLE_OK;
 }
 
 }  // namespace mole

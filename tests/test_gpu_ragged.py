@@ -101,6 +101,30 @@ def test_few_rows_long_reductions(rows, k, n):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("counts,head,tail,k,n", [
+    ([40], 0, 0, 2048, 64), ([1, 16, 17, 0, 33], 2, 90, 1000, 100), ([15], 0, 300, 4100, 72), ([0, 3], 1, 60, 8192, 33),
+    ([5000], 0, 7, 97, 146), ([0, 3001, 12], 5, 0, 64, 64), ([4096, 130], 0, 0, 264, 8), ([100], 0, 0, 1, 7)])
+def test_few_tiles_and_long_reductions(dtype, counts, head, tail, k, n):
+    """Too few tiles for the SMs: the reductions are cut into parts, over the width in the products, over
+    the rows in the weight gradient; tiles of at most 16 rows have a form of their own."""
+    from mole_b200 import ops
+    o, R, E = offs(counts, head), head + sum(counts) + tail, len(counts)
+    x, b = rnd(R, k, seed=1, dtype=dtype), rnd(R, n, seed=2, dtype=dtype)
+    x[:head], b[:head], x[R - tail:], b[R - tail:] = (float("nan"),) * 4
+    for kn in (False, True):
+        w = rnd(E, *((k, n) if kn else (n, k)), seed=3, dtype=dtype)
+        y = ops.grouped_mm(x, w, o, w_kn=kn)
+        assert not y[:head].any() and not y[R - tail:].any()
+        own = slice(head, R - tail)
+        want, mag = want_rows(x, w, o, kn)
+        close(y[own], want[own], mag[own], k, f"kn={kn}")
+        assert torch.equal(y, ops.grouped_mm(x, w, o, w_kn=kn))
+    dw = ops.grouped_mm_wgrad(x, b, o)
+    close(dw, *want_wgrad(x, b, o), max(counts), "wgrad")
+    assert torch.equal(dw, ops.grouped_mm_wgrad(x, b, o))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("k,n", [(136, 264), (72, 33)])
 def test_rows_of_others_do_not_leak(dtype, k, n):
     """NaN and infinities in the rows of one expert and of nobody stay there, also where a tile of the
