@@ -3,13 +3,15 @@
 //
 // A thread block takes a tile of T x T outputs, a thread (T / 16)^2 of them in registers; tiles of both
 // operands, 16 deep in the reduction, go through shared memory, the next ones on their way in
-// registers meanwhile.  With T = 128 a thread makes 64 multiply-adds per step on four 16-byte reads.
+// registers meanwhile.  Columns come in pairs on the packed multiply-add, the row's value twice in a
+// pair of registers: 32 instructions per step on four 16-byte reads.
 // T = 64 where experts have few rows, and 16 rows for a tile that holds no more.  Sums run over the
 // reduction in its order, one fused multiply-add after the other; where there are too few tiles for
-// the SMs the reduction is cut into parts, joined in their order by a second kernel.  Bound by the fp32 pipes: 8192 rows, 8 experts of 512 x 2048 in 0.45 ms
-// each way, 38 to 41 TFLOP/s, which is what a plain loop of library products reaches; pairs on the
-// packed instructions (0.52 ms), fragments read one step ahead and one block of twice the registers
-// per SM (0.45 to 0.5) are no faster.
+// the SMs the reduction is cut into parts, joined in their order by a second kernel.  Bound by the
+// fp32 pipes: 8192 rows over 8 experts of 512 x 2048 in 0.36 ms, dx in 0.39 and dw in 0.38 (44 to 48
+// TFLOP/s; 52 where the tiles fill the SMs evenly, a library product of the same size 55).  Single multiply-adds reach three quarters of that (they wait for shared
+// memory with the pipes 57 % busy), pairs with the row's value twice in shared memory less still.
+#include "f32x2.cuh"
 #include "ragged.cuh"
 
 namespace mole {
@@ -29,33 +31,44 @@ __device__ __forceinline__ void load8(const float* p, int n, float (&v)[8]) {
   }
 }
 
+// Four neighbouring elements, those from `n` on as zeros
+template <bool WIDE>
+__device__ __forceinline__ void load4(const float* p, int n, float (&v)[4]) {
+  if (WIDE && n >= 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : 0.f;
+  }
+}
+
 // One operand's tile: `mn` runs over T rows (or columns) of the output, k over the reduction.  KMAJOR:
 // element (mn, k) at p + mn * ld + k, else at p + k * ld + mn.
 template <int T, bool KMAJOR, bool WIDE>
 struct Operand {
-  static constexpr int kThreads = 2 * T;         // that load: T * 16 elements, eight each
-  float v[8];
+  static constexpr int kPer = T / 64;            // pieces of four that a thread loads
+  float v[kPer][4];
+  __device__ __forceinline__ int mn_of(int h) const { return KMAJOR ? (threadIdx.x >> 2) + 64 * h : threadIdx.x % (T / 4) * 4; }
+  __device__ __forceinline__ int k_of(int h) const { return KMAJOR ? (threadIdx.x & 3) * 4 : threadIdx.x / (T / 4) + 8 * h; }
   // `mn_left`, `k_left`: what exists from this tile's first element on
   __device__ __forceinline__ void fetch(const float* p, int64_t ld, int mn_left, int k_left) {
-    const int t = threadIdx.x;
-    if (t >= kThreads) return;
-    if (KMAJOR) {
-      const int mn = t % T, k = t / T * 8;
-      load8<WIDE>(p + (int64_t)mn * ld + k, mn < mn_left ? k_left - k : 0, v);
-    } else {
-      const int k = t / (T / 8), mn = t % (T / 8) * 8;
-      load8<WIDE>(p + (int64_t)k * ld + mn, k < k_left ? mn_left - mn : 0, v);
+#pragma unroll
+    for (int h = 0; h < kPer; ++h) {
+      const int mn = mn_of(h), k = k_of(h);
+      if (KMAJOR) load4<WIDE>(p + (int64_t)mn * ld + k, mn < mn_left ? k_left - k : 0, v[h]);
+      else load4<WIDE>(p + (int64_t)k * ld + mn, k < k_left ? mn_left - mn : 0, v[h]);
     }
   }
   __device__ __forceinline__ void put(float (&s)[kSK][T + 4]) const {
-    const int t = threadIdx.x;
-    if (t >= kThreads) return;
-    if (KMAJOR) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[t / T * 8 + i][t % T] = v[i];
-    } else {
+    for (int h = 0; h < kPer; ++h) {
+      if (KMAJOR) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[t / (T / 8)][t % (T / 8) * 8 + i] = v[i];
+        for (int i = 0; i < 4; ++i) s[k_of(h) + i][mn_of(h)] = v[h][i];
+      } else {
+        *reinterpret_cast<float4*>(&s[k_of(h)][mn_of(h)]) = make_float4(v[h][0], v[h][1], v[h][2], v[h][3]);
+      }
     }
   }
 };
@@ -70,6 +83,7 @@ __device__ __forceinline__ void tile_product(const float* pa, int64_t lda, int m
   constexpr int M = T / 16;
   __shared__ __align__(16) float as[2][kSK][T + 4], bs[2][kSK][T + 4];
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+  uint64_t acc2[M][M / 2] = {};
   Operand<T, A_K, WIDE> a;
   Operand<T, B_K, WIDE> b;
   a.fetch(pa, lda, m_left, K);
@@ -86,13 +100,21 @@ __device__ __forceinline__ void tile_product(const float* pa, int64_t lda, int m
     }
 #pragma unroll
     for (int k = 0; k < kSK; ++k) {
-      float x[M], y[M];
+      float x[M];
+      uint64_t y[M / 2];
 #pragma unroll
-      for (int i = 0; i < M; ++i) { x[i] = as[buf][k][tile_index<T>(ty, i)]; y[i] = bs[buf][k][tile_index<T>(tx, i)]; }
+      for (int i = 0; i < M; ++i) x[i] = as[buf][k][tile_index<T>(ty, i)];
 #pragma unroll
-      for (int i = 0; i < M; ++i)
+      for (int h = 0; h < M / 4; ++h) {
+        const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(&bs[buf][k][64 * h + 4 * tx]);
+        y[2 * h] = t.x; y[2 * h + 1] = t.y;
+      }
 #pragma unroll
-        for (int j = 0; j < M; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
+      for (int i = 0; i < M; ++i) {
+        const uint64_t xx = f2_dup(x[i]);
+#pragma unroll
+        for (int j = 0; j < M / 2; ++j) acc2[i][j] = f2_fma(xx, y[j], acc2[i][j]);
+      }
     }
     if (more) {
       a.put(as[buf ^ 1]);
@@ -100,6 +122,10 @@ __device__ __forceinline__ void tile_product(const float* pa, int64_t lda, int m
       __syncthreads();
     }
   }
+#pragma unroll
+  for (int i = 0; i < M; ++i)
+#pragma unroll
+    for (int j = 0; j < M / 2; ++j) f2_unpack(acc2[i][j], acc[i][2 * j], acc[i][2 * j + 1]);
 }
 
 // The same for a tile of at most 16 rows and 64 columns: four groups of 64 threads take a quarter of every
