@@ -93,10 +93,17 @@ void check_offsets(const at::Tensor& o, int64_t E) {
 int32_t narrow(int64_t n) {              // sizes that do not fit are refused by the C entry
   return n > INT32_MAX ? INT32_MAX : (int32_t)n;
 }
-at::Tensor output(const at::Tensor* given, const at::Tensor& like, at::IntArrayRef shape, at::ScalarType dtype) {
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  const char* x = static_cast<const char*>(a.data_ptr());
+  const char* y = static_cast<const char*>(b.data_ptr());
+  return x < y + b.nbytes() && y < x + a.nbytes();
+}
+at::Tensor output(const at::Tensor* given, const at::Tensor& like, const at::Tensor& other, at::IntArrayRef shape,
+                  at::ScalarType dtype) {
   if (given == nullptr) return at::empty(shape, like.options().dtype(dtype));
   TORCH_CHECK_VALUE(given->sizes() == shape && given->scalar_type() == dtype, "out must be ", dtype, " ", shape);
   check_with(*given, like);
+  TORCH_CHECK_VALUE(!overlap(*given, like) && !overlap(*given, other), "out overlaps an operand");
   return *given;
 }
 const at::Tensor* maybe(PyObject* o) { return o == Py_None ? nullptr : &tensor_of(o, "out"); }
@@ -112,7 +119,7 @@ at::Tensor rows_product(const at::Tensor& x, const at::Tensor& w, const at::Tens
   check_with(w, x);
   check_with(o, x);
   c10::cuda::OptionalCUDAGuard guard(x.device());
-  at::Tensor out = output(given, x, {R, N}, x.scalar_type()), ws;
+  at::Tensor out = output(given, x, w, {R, N}, x.scalar_type()), ws;
   int64_t bytes = 0;
   check_status(grouped_mm_workspace_bytes_(x.data_ptr(), w.data_ptr(), R, narrow(N), narrow(K), narrow(E), kn,
                                            (int32_t)x.element_size(), &bytes));
@@ -133,7 +140,7 @@ at::Tensor weight_gradient(const at::Tensor& a, const at::Tensor& b, const at::T
   check_with(b, a);
   check_with(o, a);
   c10::cuda::OptionalCUDAGuard guard(a.device());
-  at::Tensor out = output(given, a, {E, P, Q}, a.scalar_type()), ws;
+  at::Tensor out = output(given, a, b, {E, P, Q}, a.scalar_type()), ws;
   int64_t bytes = 0;
   check_status(grouped_mm_wgrad_workspace_bytes_(a.data_ptr(), b.data_ptr(), R, narrow(P), narrow(Q), narrow(E), dt, &bytes));
   if (bytes) ws = bytes_like(a, bytes);
@@ -243,7 +250,7 @@ PyObject* py_mm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check_with(w, q);
     check_with(ws, q);
     c10::cuda::OptionalCUDAGuard guard(q.device());
-    at::Tensor out = output(maybe(a[6]), q, {R, N}, dtype), scratch;
+    at::Tensor out = output(maybe(a[6]), q, w, {R, N}, dtype), scratch;
     int64_t bytes = 0;
     check_status(grouped_mm_workspace_bytes_(q.data_ptr(), w.data_ptr(), R, narrow(N), narrow(K), narrow(E), 0, 1, &bytes));
     if (bytes) scratch = bytes_like(q, bytes);

@@ -359,11 +359,12 @@ def test_int8_dense_and_few_rows(rows, k, n):
 def test_int8_sums_use_all_32_bits():
     """All products at their largest: 131071 times -128 times -128 is 2^31 - 2^14."""
     from mole_b200 import ops
-    for k in (131071, 131056):
-        q, w = (torch.full((n, k), -128, dtype=torch.int8, device="cuda") for n in (3, 5))
-        y = ops.mm_int8(q, torch.ones(3, device="cuda"), w, torch.ones(5, device="cuda"), out_dtype=F32)
+    for k, rows in itertools.product((131071, 131056), (3, 20)):
+        q, w = (torch.full((n, k), -128, dtype=torch.int8, device="cuda") for n in (rows, 5))
+        ones = torch.ones(20, device="cuda")
+        y = ops.mm_int8(q, ones[:rows], w, ones[:5], out_dtype=F32)
         assert (y == torch.tensor(k * 16384.0)).all()
-        y = ops.mm_int8(q, torch.ones(3, device="cuda"), torch.full_like(w, 127), torch.ones(5, device="cuda"), out_dtype=F32)
+        y = ops.mm_int8(q, ones[:rows], torch.full_like(w, 127), ones[:5], out_dtype=F32)
         assert (y == torch.tensor(float(-k * 128 * 127))).all()
 
 
@@ -494,6 +495,7 @@ def test_refusals():
             (ValueError, "different devices", lambda: ops.grouped_mm(x, w, o.cpu())),
             (RuntimeError, "CUDA tensors", lambda: ops.grouped_mm(x.cpu(), w.cpu(), o.cpu())),
             (ValueError, "out must be", lambda: ops.grouped_mm(x, w, o, out=x)),
+            (ValueError, "overlaps", lambda: ops.grouped_mm(x, rnd(2, 16, 16), o, out=x)),
             (ValueError, "takes a", lambda: ops.grouped_mm_wgrad(x, x[:5], o)),
             (ValueError, "out must be", lambda: ops.grouped_mm_wgrad(x, x, o, out=w)),
             (TypeError, "int8", lambda: ops.grouped_mm_int8(x, s, wq, ws, o)),
