@@ -28,9 +28,10 @@ __device__ __noinline__ int quantize_one(float x, float scale, float inv) {
 // V = 1: rows that 16-byte loads cannot address.
 template <typename T, int V, int G, bool HELD>
 __global__ void __launch_bounds__(256)
-quantize_rows_kernel(const T* __restrict__ x, int64_t R, int K, int8_t* __restrict__ q, float* __restrict__ scale) {
+quantize_rows_kernel(const T* x, int64_t R, int K, int8_t* __restrict__ q, float* __restrict__ scale) {
   constexpr int kHeld = 8;
   __shared__ uint32_t tops[8];
+  after_previous();
   const int64_t row = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
   if (row >= R) return;                                      // a whole warp, or the whole block
   const int t = threadIdx.x % G;
@@ -131,13 +132,12 @@ static int launch_quantize(const void* x, int64_t R, int K, void* q, float* scal
   // a warp a row while rows are short and fill the SMs, else a block a row
   const bool block = K > 32 * V * 8 || R < (int64_t)sm_count() * 16;
   const unsigned grid = (unsigned)(block ? R : (R + 7) / 8);
-  if (wide && block && K <= 256 * V * 8) quantize_rows_kernel<T, V, 256, true><<<grid, 256, 0, st>>>(xp, R, K, qp, scale);
-  else if (wide && block) quantize_rows_kernel<T, V, 256, false><<<grid, 256, 0, st>>>(xp, R, K, qp, scale);
-  else if (wide) quantize_rows_kernel<T, V, 32, true><<<grid, 256, 0, st>>>(xp, R, K, qp, scale);
-  else if (block) quantize_rows_kernel<T, 1, 256, false><<<grid, 256, 0, st>>>(xp, R, K, qp, scale);
-  else quantize_rows_kernel<T, 1, 32, false><<<grid, 256, 0, st>>>(xp, R, K, qp, scale);
-  MOLE_LAUNCH_OK();
-  return MOLE_OK;
+  auto kern = wide && block && K <= 256 * V * 8 ? quantize_rows_kernel<T, V, 256, true>
+              : wide && block                   ? quantize_rows_kernel<T, V, 256, false>
+              : wide                            ? quantize_rows_kernel<T, V, 32, true>
+              : block                           ? quantize_rows_kernel<T, 1, 256, false>
+                                                : quantize_rows_kernel<T, 1, 32, false>;
+  return launch_early(kern, dim3(grid), 256, 0, st, xp, R, K, qp, scale);
 }
 
 // ---- operands that the tensor cores cannot address, partial results ------------------------------------------------

@@ -49,54 +49,64 @@ int ragged_rows_few_i8(int out_dtype, const RaggedRows& a, cudaStream_t st);
 int ragged_rows_tc(int elem, int out_dtype, const RaggedRows& a, cudaStream_t st);
 int ragged_wgrad_tc(const RaggedWgrad& a, cudaStream_t st);
 
+// A kernel launched by launch_early is set up while the one before it in the stream finishes (1000 x 2048
+// quantised and multiplied with 2000 x 2048: 18.6 -> 14.8 us for the two); every thread calls
+// after_previous() before it touches global memory.
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename... P, typename... A>
+static int launch_early(void (*kern)(P...), dim3 grid, int block, size_t smem, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  MOLE_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...));
+  MOLE_LAUNCH_OK();
+  return MOLE_OK;
+}
+
 constexpr int kMaxRaggedExperts = 256;
 // Spans of rows: 0 = the rows before the first expert, 1 .. E = the experts, E + 1 = the rows behind
-// the last.  row0[i] .. row0[i + 1] is span i, tile0[i] the tiles of `unit` rows before it.
+// the last.  row0[i] .. row0[i + 1] is span i, tile0[i] the tiles before it (of 2^shift rows).
 struct RaggedSpans {
   int row0[kMaxRaggedExperts + 3];
   int tile0[kMaxRaggedExperts + 3];
 };
 
 // By one whole warp; the caller synchronises the block afterwards.
-__device__ __forceinline__ void load_spans(RaggedSpans& s, const int32_t* offsets, int E, int R, int unit) {
-  const int lane = threadIdx.x & 31;
-  const int n = E + 1;                               // offsets
-  const int per = (n + 31) / 32;
-  const int i0 = lane * per, i1 = min(n, i0 + per);
-  int run = 0;
-  for (int i = i0; i < i1; ++i) {
-    int o = offsets ? offsets[i] : (i == 0 ? 0 : R);
-    run = max(run, min(max(o, 0), R));
-    s.row0[i + 1] = run;
-  }
-  int before = run;                                  // running maximum over the lanes, then of those before
+__device__ __forceinline__ void load_spans(RaggedSpans& s, const int32_t* offsets, int E, int R, int shift) {
+  const int lane = threadIdx.x & 31, unit1 = (1 << shift) - 1;
+  int row = 0, tiles = 0;                            // where the spans so far end
+#pragma unroll 1
+  for (int j0 = 0; j0 < E + 2; j0 += 32) {           // a span per lane
+    const int j = j0 + lane;
+    int end = R;
+    if (j <= E) end = offsets ? min(max(offsets[j], 0), R) : j == 0 ? 0 : R;
+    if (lane == 0) end = max(end, row);
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, before, d);
-    if (lane >= d) before = max(before, v);
-  }
-  before = __shfl_up_sync(0xffffffffu, before, 1);
-  if (lane == 0) before = 0;
-  for (int i = i0; i < i1; ++i) s.row0[i + 1] = max(s.row0[i + 1], before);
-  if (lane == 0) { s.row0[0] = 0; s.row0[E + 2] = R; }
-  __syncwarp();
-  // tiles of the E + 2 spans
-  const int ns = E + 2, pers = (ns + 31) / 32;
-  const int j0 = lane * pers, j1 = min(ns, j0 + pers);
-  int sum = 0;
-  for (int j = j0; j < j1; ++j) sum += (s.row0[j + 1] - s.row0[j] + unit - 1) / unit;
-  int incl = sum;
+    for (int d = 1; d < 32; d <<= 1) {               // never before the end of an earlier one
+      const int v = __shfl_up_sync(0xffffffffu, end, d);
+      if (lane >= d) end = max(end, v);
+    }
+    int first = __shfl_up_sync(0xffffffffu, end, 1);
+    if (lane == 0) first = row;
+    int sum = (end - first + unit1) >> shift;
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += v;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += v;
+    }
+    sum += tiles;
+    if (j < E + 2) { s.row0[j + 1] = end; s.tile0[j + 1] = sum; }
+    row = __shfl_sync(0xffffffffu, end, 31);
+    tiles = __shfl_sync(0xffffffffu, sum, 31);
   }
-  int at = incl - sum;
-  for (int j = j0; j < j1; ++j) {
-    s.tile0[j] = at;
-    at += (s.row0[j + 1] - s.row0[j] + unit - 1) / unit;
-  }
-  if (lane == 31) s.tile0[ns] = incl;
+  if (lane == 0) { s.row0[0] = 0; s.tile0[0] = 0; }
 }
 // the span that holds tile t (t < tile0[E + 2]): the last one that starts at or before it
 __device__ __forceinline__ int span_of(const RaggedSpans& s, int E, int t) {

@@ -38,7 +38,7 @@ template <> struct FewIn<int8_t> {
 
 __device__ __forceinline__ uint4 load_stream(const void* p) {      // weights: read once, not kept in L1
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
@@ -127,6 +127,7 @@ few_nk_kernel(const RaggedRows a, const int split) {
   __shared__ FewSpans sp;
   __shared__ Acc part[kFewWarps][4 * kFewChunk];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  after_previous();
   const int e = find_expert(sp, a, blockIdx.y);
   const int groups = kFewWarps / split;
   const int fb = blockIdx.x * groups * 4;
@@ -200,6 +201,7 @@ few_kn_kernel(const RaggedRows a) {
   __shared__ float part[kFewWarps][kFewChunk][TILE];
   __shared__ float sum[kFewChunk][TILE];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  after_previous();
   const int e = find_expert(sp, a, blockIdx.y);
   const int q = blockIdx.x % kFewCluster, fb = blockIdx.x / kFewCluster * TILE;
   if (blockIdx.y == 0 && q == 0) zero_nobody<T>(sp, a, fb, fb + TILE);
@@ -222,7 +224,7 @@ few_kn_kernel(const RaggedRows a) {
           const uint4 t = load_stream(w + (int64_t)k * a.N);
           wv[0] = __uint_as_float(t.x); wv[1] = __uint_as_float(t.y); wv[2] = __uint_as_float(t.z); wv[3] = __uint_as_float(t.w);
         } else {
-          const uint2 t = __ldg(reinterpret_cast<const uint2*>(w + (int64_t)k * a.N));
+          const uint2 t = *reinterpret_cast<const uint2*>(w + (int64_t)k * a.N);
           wv[0] = __uint_as_float(t.x << 16); wv[1] = __uint_as_float(t.x & 0xffff0000u);
           wv[2] = __uint_as_float(t.y << 16); wv[3] = __uint_as_float(t.y & 0xffff0000u);
         }
@@ -279,10 +281,7 @@ static int launch_few(const RaggedRows& a, cudaStream_t st) {
       const bool wide = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.w) & (4 * sizeof(T) - 1)) == 0;
       const int tile = 32 * (wide ? 4 : 1);
       const dim3 grid((unsigned)((a.N + tile - 1) / tile * kFewCluster), experts);
-      if (wide) few_kn_kernel<T, 4><<<grid, 32 * kFewWarps, 0, st>>>(a);
-      else few_kn_kernel<T, 1><<<grid, 32 * kFewWarps, 0, st>>>(a);
-      MOLE_LAUNCH_OK();
-      return MOLE_OK;
+      return launch_early(wide ? few_kn_kernel<T, 4> : few_kn_kernel<T, 1>, grid, 32 * kFewWarps, 0, st, a);
     }
   }
   const bool wide = (size_t)a.K * sizeof(T) % 16 == 0 && (bases & 15) == 0;
@@ -293,10 +292,7 @@ static int launch_few(const RaggedRows& a, cudaStream_t st) {
     split *= 2;
   const int per = kFewWarps / split * 4;
   const dim3 grid((unsigned)((a.N + per - 1) / per), experts);
-  if (wide) few_nk_kernel<T, TO, true><<<grid, 32 * kFewWarps, 0, st>>>(a, split);
-  else few_nk_kernel<T, TO, false><<<grid, 32 * kFewWarps, 0, st>>>(a, split);
-  MOLE_LAUNCH_OK();
-  return MOLE_OK;
+  return launch_early(wide ? few_nk_kernel<T, TO, true> : few_nk_kernel<T, TO, false>, grid, 32 * kFewWarps, 0, st, a, split);
 }
 
 int ragged_rows_few(int dtype, const RaggedRows& a, cudaStream_t st) {

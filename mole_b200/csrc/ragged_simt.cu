@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(256, T == 128 ? 2 : 4)
 ragged_rows_kernel(const RaggedRows a) {
   constexpr int M = T / 16;
   __shared__ RaggedSpans sp;
-  if (threadIdx.x < 32) load_spans(sp, a.offsets, a.E, (int)a.R, T);
+  if (threadIdx.x < 32) load_spans(sp, a.offsets, a.E, (int)a.R, T == 128 ? 7 : 6);
   __syncthreads();
   const int tile = blockIdx.x;
   if (tile >= sp.tile0[a.E + 2]) return;

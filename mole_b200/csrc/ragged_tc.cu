@@ -46,13 +46,15 @@ struct RowsParams {
   int32_t* fault;
   int R, N, E;
   int nkb;              // stages of the reduction
+  int panel_shift;      // a panel has at most 2^panel_shift rows
+  int sorted;           // experts in the order of their row counts (more items than pairs of CTAs)
   int wide;             // rows of out are multiples of 16 bytes, its base too
   int stages;
   uint32_t stage_bytes;
 };
 
-// The experts' spans without tiles, in the order of falling row counts: the round-robin deal of the
-// items gives every pair its share of large and of small ones.
+// The experts, where there are more items than pairs in the order of falling row counts: the round-robin
+// deal of the items gives every pair its share of large and of small ones.
 struct RowsOrder {
   int row0[kMaxRaggedExperts + 3];       // as RaggedSpans
   int tile0[kMaxRaggedExperts + 3];
@@ -75,15 +77,15 @@ __device__ __forceinline__ RowsItem rows_item(const RowsOrder& o, int E, int nb,
     const int mid = (lo + hi) >> 1;
     if (o.start[mid] * nb <= item) lo = mid; else hi = mid;
   }
-  const int np = o.start[lo + 1] - o.start[lo];
-  const int local = item - o.start[lo] * nb;
-  const int pan = local % np;              // panels of a feature block are neighbours: they share weights through L2
+  const unsigned np = o.start[lo + 1] - o.start[lo], local = item - o.start[lo] * nb;
+  const unsigned blk = local / np;         // panels of a feature block are neighbours: they share weights through L2
+  const int pan = local - blk * np;
   const int e = o.order[lo];
   const int b = o.row0[e + 1], cnt = o.row0[e + 2] - b;
   const int per = ((cnt + np - 1) / np + STEP - 1) / STEP * STEP;
   w.valid = 1;
   w.e = e;
-  w.f0 = local / np * FB;
+  w.f0 = blk * FB;
   w.row0 = b + pan * per;
   w.rows = min(per, cnt - pan * per);      // may be <= 0 for a last panel: nothing to do
   w.n = (max(w.rows, 0) + STEP - 1) / STEP * STEP;
@@ -192,7 +194,6 @@ ragged_rows_tc_kernel(const __grid_constant__ RowsMaps maps, const __grid_consta
   const int cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
   const int E = p.E, nb = (p.N + FB - 1) / FB;
 
-  if (warp == 0) load_spans(*reinterpret_cast<RaggedSpans*>(&ord), p.offsets, E, p.R, 256);
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_u32(&tmem_base_s)), "r"(512u) : "memory");
@@ -211,37 +212,49 @@ ragged_rows_tc_kernel(const __grid_constant__ RowsMaps maps, const __grid_consta
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  __syncthreads();
-  for (int e = threadIdx.x; e < E; e += kRThreads) {
-    const int mine = ord.row0[e + 2] - ord.row0[e + 1];
-    int rk = 0;
-    for (int o = 0; o < E; ++o) {
-      const int other = ord.row0[o + 2] - ord.row0[o + 1];
-      rk += (other > mine) || (other == mine && o < e);
-    }
-    ord.order[rk] = (uint8_t)e;
-  }
-  __syncthreads();
-  if (warp == 0) {                                  // panels before the i-th expert of the order
-    int base = 0;
-    for (int i0 = 0; i0 < E; i0 += 32) {
-      const int i = i0 + lane;
-      int v = 0;
-      if (i < E) { const int e = ord.order[i]; v = ord.tile0[e + 2] - ord.tile0[e + 1]; }
-      int incl = v;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += u;
+  after_previous();
+  if (warp == 0) load_spans(*reinterpret_cast<RaggedSpans*>(&ord), p.offsets, E, p.R, p.panel_shift);
+  if (p.sorted) {
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += kRThreads) {
+      const int mine = ord.row0[e + 2] - ord.row0[e + 1];
+      int rk = 0;
+      for (int o = 0; o < E; ++o) {
+        const int other = ord.row0[o + 2] - ord.row0[o + 1];
+        rk += (other > mine) || (other == mine && o < e);
       }
-      if (i < E) ord.start[i] = base + incl - v;
-      base += __shfl_sync(0xffffffffu, incl, 31);
+      ord.order[rk] = (uint8_t)e;
     }
-    if (lane == 0) ord.start[E] = base;
+    __syncthreads();
+    if (warp == 0) {                                  // panels before the i-th expert of the order
+      int base = 0;
+      for (int i0 = 0; i0 < E; i0 += 32) {
+        const int i = i0 + lane;
+        int v = 0;
+        if (i < E) { const int e = ord.order[i]; v = ord.tile0[e + 2] - ord.tile0[e + 1]; }
+        int incl = v;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int u = __shfl_up_sync(0xffffffffu, incl, d);
+          if (lane >= d) incl += u;
+        }
+        if (i < E) ord.start[i] = base + incl - v;
+        base += __shfl_sync(0xffffffffu, incl, 31);
+      }
+      if (lane == 0) ord.start[E] = base;
+    }
+  } else if (warp == 0) {
+    __syncwarp();
+    for (int i = lane; i <= E; i += 32) {
+      ord.start[i] = ord.tile0[i + 1] - ord.tile0[1];
+      if (i < E) ord.order[i] = (uint8_t)i;
+    }
   }
   tcgen05_fence_before();
   __syncthreads();
-  cluster_sync_all();                               // barriers initialised, TMEM addresses there, in both CTAs
+  cluster_arrive_all();
+  const RowsItem first = rows_item<STEP, FB>(ord, E, nb, cluster_id);
+  cluster_wait_all();                               // barriers initialised, TMEM addresses there, in both CTAs
   tcgen05_fence_after();
   const uint32_t tmem_base = tmem_base_s;
 
@@ -250,9 +263,8 @@ ragged_rows_tc_kernel(const __grid_constant__ RowsMaps maps, const __grid_consta
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int item = cluster_id; ok; item += n_clusters) {
-      const RowsItem w = rows_item<STEP, FB>(ord, E, nb, item);
-      if (!w.valid) break;
+    RowsItem w = first;
+    for (int item = cluster_id; ok && w.valid; w = rows_item<STEP, FB>(ord, E, nb, item += n_clusters)) {
       if (w.n == 0) continue;
       const int h = w.n >> 1;                       // rows that this CTA stages
       const uint32_t tx = 2u * (kABytes + (uint32_t)h * 128u);
@@ -289,9 +301,8 @@ ragged_rows_tc_kernel(const __grid_constant__ RowsMaps maps, const __grid_consta
       int stage = 0, half = 0;
       uint32_t phase = 0, hph = 0;                  // hph: bit h = parity of the uses of TMEM half h so far
       bool ok = true;
-      for (int item = cluster_id; ok; item += n_clusters) {
-        const RowsItem w = rows_item<STEP, FB>(ord, E, nb, item);
-        if (!w.valid) break;
+      RowsItem w = first;
+      for (int item = cluster_id; ok && w.valid; w = rows_item<STEP, FB>(ord, E, nb, item += n_clusters)) {
         if (w.n == 0) continue;
         const bool both = DUAL && w.n > 128;
         const int h0 = both ? 0 : half;
@@ -362,9 +373,8 @@ ragged_rows_tc_kernel(const __grid_constant__ RowsMaps maps, const __grid_consta
     }
     int half = 0;
     uint32_t hph = 0;
-    for (int item = cluster_id;; item += n_clusters) {
-      const RowsItem w = rows_item<STEP, FB>(ord, E, nb, item);
-      if (!w.valid) break;
+    RowsItem w = first;
+    for (int item = cluster_id; w.valid; w = rows_item<STEP, FB>(ord, E, nb, item += n_clusters)) {
       if (w.n == 0) continue;
       const bool both = DUAL && w.n > 128;
       const int h0 = both ? 0 : half;
@@ -438,8 +448,7 @@ ragged_rows_tc_kernel(const __grid_constant__ RowsMaps maps, const __grid_consta
   if (*abort_flag) settle();
   __syncwarp();
   tcgen05_fence_before();
-  __syncthreads();
-  cluster_sync_all();          // nobody leaves while the peer may still touch its shared memory
+  cluster_meet();              // nobody leaves while the peer may still touch its shared memory
   if (warp == 1) {
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
@@ -459,26 +468,27 @@ struct WgradParams {
   int32_t* fault;
   int R, P, Q, E;
   int wide;             // rows of out are multiples of 16 bytes, its base too
+  int sorted;           // experts in the order of their row counts
   int split;            // an expert's rows are cut into so many parts,
   float* part;          // with a result [E, P, Q] each (split > 1)
 };
 struct WgradOrder {
   int row0[kMaxRaggedExperts + 3];
-  uint8_t order[kMaxRaggedExperts];      // experts by falling row counts
+  uint8_t order[kMaxRaggedExperts];      // experts, by falling row counts where there are more items than pairs
 };
 struct WgradItem {
   int valid, e, p0, q0, row0, rows, part;
 };
 __device__ __forceinline__ WgradItem wgrad_item(const WgradOrder& o, const WgradParams& p, int item) {
   WgradItem w;
-  const int qb = (p.Q + 255) / 256, per = (p.P + 255) / 256 * qb * p.split;
-  w.valid = item < p.E * per;
+  const unsigned qb = (p.Q + 255) / 256, per = (p.P + 255) / 256 * qb * p.split;
+  w.valid = item < p.E * (int)per;
   if (!w.valid) return w;
-  const int i = item / per, r = item - i * per;
+  const unsigned i = item / per, r = item - i * per, tile = r / p.split, pb = tile / qb;
   w.e = o.order[i];
-  w.part = r % p.split;
-  w.p0 = r / p.split / qb * 256;
-  w.q0 = r / p.split % qb * 256;
+  w.part = r - tile * p.split;
+  w.p0 = pb * 256;
+  w.q0 = (tile - pb * qb) * 256;
   w.row0 = o.row0[w.e + 1];
   w.rows = o.row0[w.e + 2] - w.row0;
   if (p.split > 1) {
@@ -511,9 +521,6 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   const int cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
   const int E = p.E;
 
-  // (the spans' tiles, which this kernel has no use for, lie where the ring will be)
-  RaggedSpans& spans = *reinterpret_cast<RaggedSpans*>(smem);
-  if (warp == 0) load_spans(spans, p.offsets, E, p.R, 256);
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_u32(&tmem_base_s)), "r"(512u) : "memory");
@@ -533,21 +540,30 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  after_previous();
+  // (the spans' tiles, which this kernel has no use for, lie where the ring will be)
+  RaggedSpans& spans = *reinterpret_cast<RaggedSpans*>(smem);
+  if (warp == 0) load_spans(spans, p.offsets, E, p.R, 8);
   __syncthreads();
   if (threadIdx.x < E + 3) ord.row0[threadIdx.x] = spans.row0[threadIdx.x];
   for (int e = threadIdx.x; e < E; e += kRThreads) {
-    const int mine = spans.row0[e + 2] - spans.row0[e + 1];
-    int rk = 0;
-    for (int o = 0; o < E; ++o) {
-      const int other = spans.row0[o + 2] - spans.row0[o + 1];
-      rk += (other > mine) || (other == mine && o < e);
+    int rk = e;
+    if (p.sorted) {
+      const int mine = spans.row0[e + 2] - spans.row0[e + 1];
+      rk = 0;
+      for (int o = 0; o < E; ++o) {
+        const int other = spans.row0[o + 2] - spans.row0[o + 1];
+        rk += (other > mine) || (other == mine && o < e);
+      }
     }
     ord.order[rk] = (uint8_t)e;
   }
   fence_async_proxy();                              // the ring's first loads overwrite the spans
   tcgen05_fence_before();
   __syncthreads();
-  cluster_sync_all();
+  cluster_arrive_all();
+  const WgradItem first = wgrad_item(ord, p, cluster_id);
+  cluster_wait_all();
   tcgen05_fence_after();
   const uint32_t tmem_base = tmem_base_s;
 
@@ -556,9 +572,8 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int item = cluster_id; ok; item += n_clusters) {
-      const WgradItem w = wgrad_item(ord, p, item);
-      if (!w.valid) break;
+    WgradItem w = first;
+    for (int item = cluster_id; ok && w.valid; w = wgrad_item(ord, p, item += n_clusters)) {
       const int c0 = (lane < 2 ? w.p0 : w.q0) + 128 * (int)rank + 64 * (lane & 1);
       for (int r = 0; r < w.rows; r += 64) {
         ok = warp_all_wait(empty0 + 8 * stage, phase ^ 1, abort_flag, p.fault, 71);
@@ -587,9 +602,8 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int item = cluster_id; ok; item += n_clusters) {
-        const WgradItem w = wgrad_item(ord, p, item);
-        if (!w.valid) break;
+      WgradItem w = first;
+      for (int item = cluster_id; ok && w.valid; w = wgrad_item(ord, p, item += n_clusters)) {
         if (w.rows == 0) continue;
         if (!(ok = mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag, p.fault, 72))) break;
         tcgen05_fence_after();
@@ -625,9 +639,8 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     // ---- fixer (both CTAs): zeros over the rows of others in an expert's last 16-row step ----
     int stage = 0;
     uint32_t seen = 0;                              // bit s: parity of the uses of part0[s] so far
-    for (int item = cluster_id;; item += n_clusters) {
-      const WgradItem w = wgrad_item(ord, p, item);
-      if (!w.valid) break;
+    WgradItem w = first;
+    for (int item = cluster_id; w.valid; w = wgrad_item(ord, p, item += n_clusters)) {
       if (w.rows == 0) continue;
       const int n = (w.rows + 63) / 64;
       const int last = (stage + n - 1) % kWStages;
@@ -653,9 +666,8 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
     uint8_t* strip = smem + kWStages * kWStageBytes + (warp - 4) * kWStripBytes;
     int turn = 0;
     uint32_t acc_phase = 0;
-    for (int item = cluster_id;; item += n_clusters) {
-      const WgradItem w = wgrad_item(ord, p, item);
-      if (!w.valid) break;
+    WgradItem w = first;
+    for (int item = cluster_id; w.valid; w = wgrad_item(ord, p, item += n_clusters)) {
       const bool empty = w.rows == 0;               // no rows: the gradient is zero
       if (empty ? ((item / n_clusters) & 1) != acc : turn != acc) {
         if (!empty) turn ^= 1;
@@ -746,8 +758,7 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   if (*abort_flag) settle();
   __syncwarp();
   tcgen05_fence_before();
-  __syncthreads();
-  cluster_sync_all();
+  cluster_meet();
   if (warp == 1) {
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
@@ -795,11 +806,10 @@ static int launch_rows(const RowsMaps& maps, RowsParams p, int n_max, int64_t pa
   static PerDeviceInt cache;
   int pairs = 0;
   if (int rc = resident_pairs(kern, kRBudget, cache, &pairs)) return rc;
+  p.sorted = max_items > pairs;
   if (max_items < pairs) pairs = (int)max_items;
   const size_t smem = (size_t)p.stages * p.stage_bytes + 1024;
-  kern<<<2 * pairs, kRThreads, smem, st>>>(maps, p);
-  MOLE_LAUNCH_OK();
-  return MOLE_OK;
+  return launch_early(kern, dim3(2 * pairs), kRThreads, smem, st, maps, p);
 }
 
 int ragged_rows_tc(int elem, int out_dtype, const RaggedRows& a, cudaStream_t st) {
@@ -821,10 +831,16 @@ int ragged_rows_tc(int elem, int out_dtype, const RaggedRows& a, cudaStream_t st
   p.nkb = (int)((a.K + kb - 1) / kb);
   const size_t osize = out_dtype == MOLE_F32 ? 4 : 2;
   p.wide = a.N * osize % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
-  // no panel has more than min(256, R) rows: few rows leave the shared memory to more stages
+  // panels of 256 rows, of half as many as long as all items still run at once (1000 rows, 2048 -> 2000 in 8
+  // bits: 64 items of 128 rows, 11.1 us; 32 of 256, 11.8)
   const int step = elem == 1 ? 32 : 16;
-  const int n_max = a.R >= 256 ? 256 : (int)((a.R + step - 1) / step * step);
-  const int64_t panels = a.R / 256 + (a.E < a.R ? a.E : a.R);       // every expert may end in a partial one
+  auto panels_of = [&](int panel) { return a.R / panel + (a.E < a.R ? a.E : a.R); };  // every expert may end in a partial one
+  int panel = 256;
+  while (panel > 32 && panels_of(panel / 2) * ((a.N + 255) / 256) <= sm_count() / 2) panel /= 2;
+  p.panel_shift = panel == 256 ? 8 : panel == 128 ? 7 : panel == 64 ? 6 : 5;
+  const int64_t panels = panels_of(panel);
+  // no panel has more rows than there are: few rows leave the shared memory to more stages
+  const int n_max = a.R >= panel ? panel : (int)((a.R + step - 1) / step * step);
   // 512 features per item where that still leaves every pair two items or so, and the last block is not
   // mostly empty: 64 experts of 256 rows, 8192 -> 2048: 0.49 ms, with 256 features 0.63; 1000 rows of one
   // expert, 2048 -> 2000 in 8 bits: 20 us, with 256 features 13
@@ -862,6 +878,7 @@ int ragged_wgrad_tc(const RaggedWgrad& a, cudaStream_t st) {
   p.part = a.part;
   const int64_t items = (int64_t)a.E * a.split * ((a.P + 255) / 256) * ((a.Q + 255) / 256);
   MOLE_REQUIRE(items < (1ll << 31), "%d experts of %d x %d", a.E, a.P, a.Q);
+  p.sorted = items > pairs;
   if (items < pairs) pairs = (int)items;
   CUtensorMap mo = ma;
   if (p.wide) {
@@ -869,8 +886,7 @@ int ragged_wgrad_tc(const RaggedWgrad& a, cudaStream_t st) {
     const uint32_t box_out[3] = {32, 32, 1};
     if (int rc = encode_map(&mo, a.out, 3, dims, box_out, 2)) return rc;
   }
-  ragged_wgrad_tc_kernel<<<2 * pairs, kRThreads, smem, st>>>(ma, mb, mo, p);
-  MOLE_LAUNCH_OK();
+  if (int rc = launch_early(ragged_wgrad_tc_kernel, dim3(2 * pairs), kRThreads, smem, st, ma, mb, mo, p)) return rc;
   return a.split > 1 ? ragged_join(MOLE_BF16, a.part, a.split, (int64_t)a.E * a.P * a.Q, a.out, st) : MOLE_OK;
 }
 
