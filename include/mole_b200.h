@@ -307,9 +307,10 @@ int mole_ffn_bwd_peer(const mole_ffn_desc* desc, const int32_t* counts,
  * the device, as mole_gate_route_fwd writes them; E <= 256; an expert may have no rows).  Rows before
  * offsets[0] and from offsets[E] on belong to nobody: products write zeros there.  The offsets are
  * clamped on the device to a rising sequence in [0, R].  Any width and element-aligned pointers are
- * taken; operands of bf16 and 8-bit integers whose rows do not start on 16 bytes are first copied
- * into the workspace, whose size mole_grouped_mm_workspace_bytes gives (0, and null will do, where
- * all rows do, for fp32, and for up to 16 rows).  All sums are held in 32 bits and rounded once.
+ * taken.  The workspace (its size from the _workspace_bytes calls; null will do for 0) holds copies of
+ * bf16 and 8-bit operands whose rows do not start on 16 bytes, and partial results where a product
+ * has too few tiles for the SMs and its reduction is cut into parts; 0 for up to 16 rows.  All sums are
+ * held in 32 bits, parts are joined in their order, and a result is rounded once.
  * The reference computes the same products inside bffn_fwd / bffn_bwd over capacity-padded rows
  * (MOLE/cpp/core.cpp:350-353, 388-412).
  * ---------------------------------------------------------------------------------- */

@@ -11,7 +11,8 @@ namespace mole {
 // quotient t is taken as x * (1 / scale), which is off by less than 2^-23 of 127; where that leaves
 // doubt about the nearest integer (1 value in 10^4), the sign of x - (n + 1/2) scale decides, which
 // one fused multiply-add gives exactly.  (A call: inlined 64 times, the kernel misses in the instruction
-// cache.)
+// cache.)  Bound by instructions, not by HBM's 3 bytes an element: 32768 x 2048 of bf16 in 53 us (3.8 TB/s;
+// 76 with a division each).
 __device__ __noinline__ int quantize_one(float x, float scale, float inv) {
   const float t = x * inv;
   float r = rintf(t);
@@ -140,11 +141,12 @@ static int launch_quantize(const void* x, int64_t R, int K, void* q, float* scal
   return launch_early(kern, dim3(grid), 256, 0, st, xp, R, K, qp, scale);
 }
 
-// ---- operands that the tensor cores cannot address, partial results ------------------------------------------------
+// ---- operands that the tensor cores cannot address, partial results ---------------------------
 // TMA wants rows that start on 16 bytes.  Operands of other widths or at other addresses are copied to
 // rows that do, in the caller's workspace; the copy costs a pass of HBM over the operand (weights:
 // only those of experts that have rows), the products on the CUDA cores an order of magnitude.
-// A thread makes 16 bytes of the copy from two aligned pieces; matrix m of `rows` rows belongs to expert m, one matrix belongs to all.
+// A thread makes 16 bytes of the copy from two aligned pieces.  Matrix m of `rows` rows belongs to expert
+// m; a single matrix belongs to all.  (1237 rows of 13 experts, 1001 x 328: dx 105 -> 14 us, dw 83 -> 16.)
 __global__ void __launch_bounds__(256)
 align_rows_kernel(const uint8_t* __restrict__ src, int64_t rows, int row_bytes, int ld_bytes, uint8_t* __restrict__ dst,
                   const int32_t* __restrict__ offsets) {

@@ -3,7 +3,8 @@
 // With that few rows a product is one reading of the weights of the experts that have rows: 2 N K
 // bytes of bf16 per expert, a row's worth of multiply-adds on each, which the CUDA cores keep up with.
 // What counts is loads in flight.  The tensor-core kernel gives a decode step one pair of SMs per
-// 256 features (64 pairs at best, and a pipeline to fill); here every warp of every SM streams weights.
+// 256 features (64 pairs at best, and a pipeline to fill); here every warp of every SM streams weights:
+// one token with two of 64 experts of 2048 x 8192 takes 15 us (67 MB at 4.5 TB/s), there 22.
 //
 // K-major weights (few_nk): a warp takes four features, its lanes run along the reduction with 16-byte
 // loads; up to eight warps share the reduction of the same features when there are few of them.

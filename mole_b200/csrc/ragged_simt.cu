@@ -8,9 +8,10 @@
 // T = 64 where experts have few rows, and 16 rows for a tile that holds no more.  Sums run over the
 // reduction in its order, one fused multiply-add after the other; where there are too few tiles for
 // the SMs the reduction is cut into parts, joined in their order by a second kernel.  Bound by the
-// fp32 pipes: 8192 rows over 8 experts of 512 x 2048 in 0.36 ms, dx in 0.39 and dw in 0.38 (44 to 48
-// TFLOP/s; 52 where the tiles fill the SMs evenly, a library product of the same size 55).  Single multiply-adds reach three quarters of that (they wait for shared
-// memory with the pipes 57 % busy), pairs with the row's value twice in shared memory less still.
+// fp32 pipes: 8192 rows over 8 experts of 512 x 2048 in 0.38 ms, dx in 0.37 and dw in 0.38 (45 to 46
+// TFLOP/s; 52 where the tiles fill the SMs evenly, a library product of the same size 55).  Single
+// multiply-adds reach three quarters of that (they wait for shared memory with the pipes 57 % busy),
+// pairs with the row's value twice in shared memory less still.
 #include "f32x2.cuh"
 #include "ragged.cuh"
 
