@@ -1,17 +1,18 @@
 // fp32 products over rows packed by expert, on the CUDA cores: they have to be exact to 2^-24, which the
 // tensor cores' input types are not.  Every size and alignment.
 //
-// A thread block takes a tile of T x T outputs, a thread (T / 16)^2 of them in registers; tiles of both
-// operands, 16 deep in the reduction, go through shared memory, the next ones on their way in
-// registers meanwhile.  Columns come in pairs on the packed multiply-add, the row's value twice in a
-// pair of registers: 32 instructions per step on four 16-byte reads.
+// A thread block takes a tile of T x T outputs, a thread 16 x 8 of them in registers (4 x 4 for T = 64);
+// tiles of both operands, 16 deep in the reduction, go through shared memory, the next ones on their way
+// in registers meanwhile.  Rows come in pairs on the packed multiply-add, the column's value twice in
+// a pair of registers: 64 instructions per step on six 16-byte reads, which shared memory serves in 24
+// cycles a warp, the multiply-adds in 32 (of four warps at a time).  With 8 x 8 it is 32 on four, both
+// take the same time, and the kernel a tenth longer; with pairs along the reduction in 8 x 4 (no value
+// twice, but six reads for 32) a fifth longer still.
 // T = 64 where experts have few rows, and 16 rows for a tile that holds no more.  Sums run over the
 // reduction in its order, one fused multiply-add after the other; where there are too few tiles for
 // the SMs the reduction is cut into parts, joined in their order by a second kernel.  Bound by the
-// fp32 pipes: 8192 rows over 8 experts of 512 x 2048 in 0.38 ms, dx in 0.37 and dw in 0.38 (45 to 46
-// TFLOP/s; 52 where the tiles fill the SMs evenly, a library product of the same size 55).  Single
-// multiply-adds reach three quarters of that (they wait for shared memory with the pipes 57 % busy),
-// pairs with the row's value twice in shared memory less still.
+// fp32 pipes: 8192 rows over 8 experts of 512 x 2048 in 0.35 ms, dx in 0.37 and dw in 0.35 (46 to 49
+// TFLOP/s; 56 where the tiles fill the SMs evenly, a library product of the same size 55).
 #include "f32x2.cuh"
 #include "ragged.cuh"
 
@@ -44,14 +45,25 @@ __device__ __forceinline__ void load4(const float* p, int n, float (&v)[4]) {
   }
 }
 
+// Tiles of T x T outputs: `kThreads` threads, kRows x kCols outputs each
+template <int T>
+struct Tile {
+  static constexpr int kThreads = T == 128 ? 128 : 256;
+  static constexpr int kRows = T == 128 ? 16 : 4, kCols = T * T / kThreads / kRows;
+  static constexpr int kRowStep = kThreads / 16 * 4;       // rows of a thread come in fours, so far apart
+  __device__ static __forceinline__ int row(int i) { return (i >> 2) * kRowStep + (threadIdx.x >> 4) * 4 + (i & 3); }
+  __device__ static __forceinline__ int col(int j) { return (j >> 2) * 64 + (threadIdx.x & 15) * 4 + (j & 3); }
+};
+
 // One operand's tile: `mn` runs over T rows (or columns) of the output, k over the reduction.  KMAJOR:
 // element (mn, k) at p + mn * ld + k, else at p + k * ld + mn.
 template <int T, bool KMAJOR, bool WIDE>
 struct Operand {
-  static constexpr int kPer = T / 64;            // pieces of four that a thread loads
+  static constexpr int kThreads = Tile<T>::kThreads;
+  static constexpr int kPer = T * kSK / 4 / kThreads;      // pieces of four that a thread loads
   float v[kPer][4];
-  __device__ __forceinline__ int mn_of(int h) const { return KMAJOR ? (threadIdx.x >> 2) + 64 * h : threadIdx.x % (T / 4) * 4; }
-  __device__ __forceinline__ int k_of(int h) const { return KMAJOR ? (threadIdx.x & 3) * 4 : threadIdx.x / (T / 4) + 8 * h; }
+  __device__ __forceinline__ int mn_of(int h) const { return KMAJOR ? (threadIdx.x >> 2) + kThreads / 4 * h : threadIdx.x % (T / 4) * 4; }
+  __device__ __forceinline__ int k_of(int h) const { return KMAJOR ? (threadIdx.x & 3) * 4 : threadIdx.x / (T / 4) + kThreads / (T / 4) * h; }
   // `mn_left`, `k_left`: what exists from this tile's first element on
   __device__ __forceinline__ void fetch(const float* p, int64_t ld, int mn_left, int k_left) {
 #pragma unroll
@@ -75,16 +87,13 @@ struct Operand {
 };
 
 // acc = A (T x K) B (K x T); pa and pb point to the tile's first elements at k = 0.  Output (i, j) of a
-// thread is row row_of(i), column col_of(j) of the tile.
-template <int T>
-__device__ __forceinline__ int tile_index(int t16, int i) { return (i >> 2) * 64 + t16 * 4 + (i & 3); }
+// thread is row Tile<T>::row(i), column Tile<T>::col(j) of the tile.
 template <int T, bool A_K, bool B_K, bool WIDE>
 __device__ __forceinline__ void tile_product(const float* pa, int64_t lda, int m_left, const float* pb, int64_t ldb,
-                                             int n_left, int K, float (&acc)[T / 16][T / 16]) {
-  constexpr int M = T / 16;
+                                             int n_left, int K, float (&acc)[Tile<T>::kRows][Tile<T>::kCols]) {
+  constexpr int M = Tile<T>::kRows, N = Tile<T>::kCols;
   __shared__ __align__(16) float as[2][kSK][T + 4], bs[2][kSK][T + 4];
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  uint64_t acc2[M][M / 2] = {};
+  uint64_t acc2[M / 2][N] = {};                            // of two neighbouring rows
   Operand<T, A_K, WIDE> a;
   Operand<T, B_K, WIDE> b;
   a.fetch(pa, lda, m_left, K);
@@ -101,20 +110,23 @@ __device__ __forceinline__ void tile_product(const float* pa, int64_t lda, int m
     }
 #pragma unroll
     for (int k = 0; k < kSK; ++k) {
-      float x[M];
-      uint64_t y[M / 2];
+      uint64_t x[M / 2];
+      float y[N];
 #pragma unroll
-      for (int i = 0; i < M; ++i) x[i] = as[buf][k][tile_index<T>(ty, i)];
-#pragma unroll
-      for (int h = 0; h < M / 4; ++h) {
-        const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(&bs[buf][k][64 * h + 4 * tx]);
-        y[2 * h] = t.x; y[2 * h + 1] = t.y;
+      for (int i = 0; i < M; i += 4) {
+        const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(&as[buf][k][Tile<T>::row(i)]);
+        x[i / 2] = t.x; x[i / 2 + 1] = t.y;
       }
 #pragma unroll
-      for (int i = 0; i < M; ++i) {
-        const uint64_t xx = f2_dup(x[i]);
+      for (int j = 0; j < N; j += 4) {
+        const float4 t = *reinterpret_cast<const float4*>(&bs[buf][k][Tile<T>::col(j)]);
+        y[j] = t.x; y[j + 1] = t.y; y[j + 2] = t.z; y[j + 3] = t.w;
+      }
 #pragma unroll
-        for (int j = 0; j < M / 2; ++j) acc2[i][j] = f2_fma(xx, y[j], acc2[i][j]);
+      for (int j = 0; j < N; ++j) {
+        const uint64_t yy = f2_dup(y[j]);
+#pragma unroll
+        for (int i = 0; i < M / 2; ++i) acc2[i][j] = f2_fma(x[i], yy, acc2[i][j]);
       }
     }
     if (more) {
@@ -124,9 +136,9 @@ __device__ __forceinline__ void tile_product(const float* pa, int64_t lda, int m
     }
   }
 #pragma unroll
-  for (int i = 0; i < M; ++i)
+  for (int i = 0; i < M / 2; ++i)
 #pragma unroll
-    for (int j = 0; j < M / 2; ++j) f2_unpack(acc2[i][j], acc[i][2 * j], acc[i][2 * j + 1]);
+    for (int j = 0; j < N; ++j) f2_unpack(acc2[i][j], acc[2 * i][j], acc[2 * i + 1][j]);
 }
 
 // The same for a tile of at most 16 rows and 64 columns: four groups of 64 threads take a quarter of every
@@ -201,10 +213,22 @@ __device__ __forceinline__ void put4(float* d, const float* v, int left, bool ve
   }
 }
 
+// The tile's outputs; `m_left`, `n_left` of its rows and columns exist
+template <int T>
+__device__ __forceinline__ void put_tile(float* out, int64_t ld, int m_left, int n_left,
+                                         const float (&acc)[Tile<T>::kRows][Tile<T>::kCols], bool vec) {
+#pragma unroll
+  for (int i = 0; i < Tile<T>::kRows; ++i) {
+    const int r = Tile<T>::row(i);
+    if (r >= m_left) continue;
+#pragma unroll
+    for (int j = 0; j < Tile<T>::kCols; j += 4) put4(out + r * ld + Tile<T>::col(j), &acc[i][j], n_left - Tile<T>::col(j), vec);
+  }
+}
+
 template <int T, bool KN, bool WIDE>
-__global__ void __launch_bounds__(256, T == 128 ? 2 : 4)
+__global__ void __launch_bounds__(Tile<T>::kThreads, T == 128 ? 2 : 4)
 ragged_rows_kernel(const RaggedRows a) {
-  constexpr int M = T / 16;
   __shared__ RaggedSpans sp;
   if (threadIdx.x < 32) load_spans(sp, a.offsets, a.E, (int)a.R, T == 128 ? 7 : 6);
   __syncthreads();
@@ -220,7 +244,7 @@ ragged_rows_kernel(const RaggedRows a) {
   const bool vec = a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   const int e = span - 1;
   const bool owned = e >= 0 && e < a.E;
-  float acc[M][M] = {};
+  float acc[Tile<T>::kRows][Tile<T>::kCols] = {};
   if (owned) {
     const float* x = static_cast<const float*>(a.x) + (int64_t)r0 * a.K + k0;
     const float* w = static_cast<const float*>(a.w) + (int64_t)e * a.N * a.K + (KN ? (int64_t)k0 * a.N : (int64_t)k0);
@@ -240,17 +264,7 @@ ragged_rows_kernel(const RaggedRows a) {
     }
     if (len > 0) tile_product<T, true, !KN, WIDE>(x, a.K, rend - r0, wt, ldw, a.N - n0, len, acc);
   }
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-#pragma unroll
-  for (int i = 0; i < M; ++i) {
-    const int r = r0 + tile_index<T>(ty, i);
-    if (r >= rend) continue;
-#pragma unroll
-    for (int j = 0; j < M; j += 4) {
-      const int n = n0 + tile_index<T>(tx, j);
-      put4(out + (int64_t)r * a.N + n, &acc[i][j], a.N - n, vec);
-    }
-  }
+  put_tile<T>(out + (int64_t)r0 * a.N + n0, a.N, rend - r0, a.N - n0, acc, vec);
 }
 
 // Rows of one expert, by a whole block: the running maximum over the offsets before it only where they do
@@ -259,36 +273,30 @@ __device__ __forceinline__ void expert_rows(const int32_t* offsets, int E, int R
   auto at = [&](int i) { return min(max(offsets[i], 0), R); };
   first = at(e);
   end = at(e + 1);
-  if (__syncthreads_or(threadIdx.x < E && offsets[threadIdx.x + 1] < offsets[threadIdx.x])) {
+  bool falls = false;
+  for (int i = threadIdx.x; i < E; i += blockDim.x) falls |= offsets[i + 1] < offsets[i];
+  if (__syncthreads_or(falls)) {
     for (int i = 0; i < e; ++i) first = max(first, at(i));
     end = max(first, end);
   }
 }
 
 template <int T, bool WIDE>
-__global__ void __launch_bounds__(256, T == 128 ? 2 : 4)
+__global__ void __launch_bounds__(Tile<T>::kThreads, T == 128 ? 2 : 4)
 ragged_wgrad_kernel(const RaggedWgrad a) {
-  constexpr int M = T / 16;
   const int e = blockIdx.z / a.split, part = blockIdx.z % a.split, q0 = blockIdx.x * T, p0 = blockIdx.y * T;
   int first, end;
   expert_rows(a.offsets, a.E, (int)a.R, e, first, end);
   const int all = end - first;
   const int share = (all + a.split * kSK - 1) / (a.split * kSK) * kSK;    // of an expert's rows per part
   const int r0 = first + part * share, rows = min(share, all - part * share);
-  float acc[M][M] = {};
+  float acc[Tile<T>::kRows][Tile<T>::kCols] = {};
   if (rows > 0)
     tile_product<T, false, false, WIDE>(static_cast<const float*>(a.a) + (int64_t)r0 * a.P + p0, a.P, a.P - p0,
                                             static_cast<const float*>(a.b) + (int64_t)r0 * a.Q + q0, a.Q, a.Q - q0, rows, acc);
   float* out = (a.split > 1 ? a.part + (int64_t)part * a.E * a.P * a.Q : static_cast<float*>(a.out)) + (int64_t)e * a.P * a.Q;
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   const bool vec = a.Q % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-#pragma unroll
-  for (int i = 0; i < M; ++i)
-#pragma unroll
-    for (int j = 0; j < M; j += 4) {
-      const int p = p0 + tile_index<T>(ty, i), q = q0 + tile_index<T>(tx, j);
-      if (p < a.P) put4(out + (int64_t)p * a.Q + q, &acc[i][j], a.Q - q, vec);
-    }
+  put_tile<T>(out + (int64_t)p0 * a.Q + q0, a.Q, a.P - p0, a.Q - q0, acc, vec);
 }
 
 // rows that start on 16 bytes
@@ -351,10 +359,10 @@ static int launch_rows(const RaggedRows& a, cudaStream_t st) {
   auto grid = [&](int T) {                                                   // every span may end in a partial tile
     return dim3((unsigned)(a.R / T + a.E + 2), (unsigned)((a.N + T - 1) / T), (unsigned)a.split);
   };
-  if (large && wide) ragged_rows_kernel<128, KN, true><<<grid(128), 256, 0, st>>>(a);
-  else if (large) ragged_rows_kernel<128, KN, false><<<grid(128), 256, 0, st>>>(a);
-  else if (wide) ragged_rows_kernel<64, KN, true><<<grid(64), 256, 0, st>>>(a);
-  else ragged_rows_kernel<64, KN, false><<<grid(64), 256, 0, st>>>(a);
+  if (large && wide) ragged_rows_kernel<128, KN, true><<<grid(128), Tile<128>::kThreads, 0, st>>>(a);
+  else if (large) ragged_rows_kernel<128, KN, false><<<grid(128), Tile<128>::kThreads, 0, st>>>(a);
+  else if (wide) ragged_rows_kernel<64, KN, true><<<grid(64), Tile<64>::kThreads, 0, st>>>(a);
+  else ragged_rows_kernel<64, KN, false><<<grid(64), Tile<64>::kThreads, 0, st>>>(a);
   MOLE_LAUNCH_OK();
   return MOLE_OK;
 }
@@ -368,10 +376,10 @@ int ragged_wgrad_simt(const RaggedWgrad& a, cudaStream_t st) {
   auto grid = [&](int T) { return dim3((unsigned)((a.Q + T - 1) / T), (unsigned)((a.P + T - 1) / T), (unsigned)(a.E * a.split)); };
   const dim3 g = grid(128);
   const bool large = wgrad_tile(a) == 128;
-  if (large && wide) ragged_wgrad_kernel<128, true><<<g, 256, 0, st>>>(a);
-  else if (large) ragged_wgrad_kernel<128, false><<<g, 256, 0, st>>>(a);
-  else if (wide) ragged_wgrad_kernel<64, true><<<grid(64), 256, 0, st>>>(a);
-  else ragged_wgrad_kernel<64, false><<<grid(64), 256, 0, st>>>(a);
+  if (large && wide) ragged_wgrad_kernel<128, true><<<g, Tile<128>::kThreads, 0, st>>>(a);
+  else if (large) ragged_wgrad_kernel<128, false><<<g, Tile<128>::kThreads, 0, st>>>(a);
+  else if (wide) ragged_wgrad_kernel<64, true><<<grid(64), Tile<64>::kThreads, 0, st>>>(a);
+  else ragged_wgrad_kernel<64, false><<<grid(64), Tile<64>::kThreads, 0, st>>>(a);
   MOLE_LAUNCH_OK();
   return a.split > 1 ? ragged_join(MOLE_F32, a.part, a.split, (int64_t)a.E * a.P * a.Q, a.out, st) : MOLE_OK;
 }
