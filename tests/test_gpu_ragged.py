@@ -438,6 +438,44 @@ def test_on_another_stream_and_two_at_once():
     assert all(torch.equal(want, y) for ys in outs for y in ys[:5]) and torch.equal(outs[0][5], outs[1][5])
 
 
+@pytest.mark.parametrize("rows", [9, 700, 5000])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_calls_back_to_back_see_what_the_one_before_wrote(dtype, rows):
+    """Inputs rewritten and outputs consumed right before and behind each call, without a pause, give the bits
+    that the same calls give one at a time."""
+    from mole_b200 import ops
+    E, K, N = 5, 256, 512
+    w1, w2 = rnd(E, N, K, seed=1, dtype=dtype, std=0.06), rnd(E, K, N, seed=2, dtype=dtype, std=0.06)
+    q1, s1 = ops.quantize_rows(w1)
+    news = [rnd(rows, K, seed=10 + i, dtype=dtype) for i in range(8)]
+    cuts = [offs([(rows * c) // 40 for c in (i, 8, 2 * i, 0, 16 - i)], head=i) for i in range(8)]
+
+    def chain(pause):
+        x, o = torch.empty_like(news[0]), torch.empty_like(cuts[0])
+        outs = []
+        for xi, oi in zip(news, cuts):
+            x.copy_(xi)
+            o.copy_(oi)
+            for f in (lambda: ops.grouped_mm(x, w1, o), lambda: ops.grouped_mm(outs[-1], w2, o),
+                      lambda: ops.grouped_mm(outs[-1], w2, o, w_kn=True), lambda: ops.grouped_mm_wgrad(outs[-1], x, o),
+                      lambda: ops.grouped_mm(outs[-4], outs[-1], o, w_kn=True),
+                      lambda: ops.quantize_rows(outs[-4])):
+                if pause:
+                    torch.cuda.synchronize()
+                got = f()
+                outs += got if isinstance(got, tuple) else [got]
+            if pause:
+                torch.cuda.synchronize()
+            outs.append(ops.grouped_mm_int8(outs[-2], outs[-1], q1, s1, o, out_dtype=dtype))
+            if pause:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return outs
+    chain(False)
+    want, got = chain(True), chain(False)
+    assert len(got) == 8 * 8 and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_captured_and_replayed_with_new_rows_and_offsets():
     import mole_b200
     from mole_b200 import ops
