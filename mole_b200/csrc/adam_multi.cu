@@ -500,6 +500,7 @@ adam_multi_kernel(const __grid_constant__ AdamTable<CAP> table, const __grid_con
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
+  after_previous();
   const int steps = (a.chunks - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
 
   struct Place { int entry, end; };                 // entry of a chunk, first chunk behind that entry
@@ -667,9 +668,7 @@ static int adam_launch(const mole_adam_tensor* t, int from, int to, AdamMulti a,
   int64_t grid = (int64_t)sm_count() * S::kResident;
   if (grid < (chunks + kAdamWalk - 1) / kAdamWalk) grid = (chunks + kAdamWalk - 1) / kAdamWalk;
   if (grid > chunks) grid = chunks;
-  kern<<<(unsigned)grid, kAdamThreads, smem, st>>>(table, a);
-  MOLE_LAUNCH_OK();
-  return MOLE_OK;
+  return launch_early(kern, dim3((unsigned)grid), kAdamThreads, smem, st, table, a);
 }
 
 template <typename T, int BITS>

@@ -49,27 +49,6 @@ int ragged_rows_few_i8(int out_dtype, const RaggedRows& a, cudaStream_t st);
 int ragged_rows_tc(int elem, int out_dtype, const RaggedRows& a, cudaStream_t st);
 int ragged_wgrad_tc(const RaggedWgrad& a, cudaStream_t st);
 
-// A kernel launched by launch_early is set up while the one before it in the stream finishes (1000 x 2048
-// quantised and multiplied with 2000 x 2048: 18.6 -> 14.8 us for the two); every thread calls
-// after_previous() before it touches global memory.
-__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-template <typename... P, typename... A>
-static int launch_early(void (*kern)(P...), dim3 grid, int block, size_t smem, cudaStream_t st, const A&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(block);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  MOLE_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...));
-  MOLE_LAUNCH_OK();
-  return MOLE_OK;
-}
-
 constexpr int kMaxRaggedExperts = 256;
 // Spans of rows: 0 = the rows before the first expert, 1 .. E = the experts, E + 1 = the rows behind
 // the last.  row0[i] .. row0[i + 1] is span i, tile0[i] the tiles before it (of 2^shift rows).
