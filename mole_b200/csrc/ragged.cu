@@ -148,8 +148,8 @@ static int launch_quantize(const void* x, int64_t R, int K, void* q, float* scal
 // A thread makes 16 bytes of the copy from two aligned pieces.  Matrix m of `rows` rows belongs to expert
 // m; a single matrix belongs to all.  (1237 rows of 13 experts, 1001 x 328: dx 105 -> 14 us, dw 83 -> 16.)
 __global__ void __launch_bounds__(256)
-align_rows_kernel(const uint8_t* __restrict__ src, int64_t rows, int row_bytes, int ld_bytes, uint8_t* __restrict__ dst,
-                  const int32_t* __restrict__ offsets) {
+align_rows_kernel(const uint8_t* src, int64_t rows, int row_bytes, int ld_bytes, uint8_t* dst, const int32_t* offsets) {
+  after_previous();
   if (offsets != nullptr && offsets[blockIdx.y + 1] <= offsets[blockIdx.y]) return;
   const int per_row = ld_bytes / 16;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -213,9 +213,9 @@ static int align_operand(Aligner& ws, const void** p, int64_t matrices, int64_t 
                "workspace of %lld bytes, %lld needed (mole_grouped_mm_workspace_bytes)", (long long)ws.left, (long long)ws.used);
   void* dst = ws.at + ws.used - bytes;
   const dim3 grid((unsigned)((rows * (*ld / unit) + 255) / 256), (unsigned)matrices);
-  align_rows_kernel<<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(*p), rows, cols * elem, *ld * elem,
-                                          static_cast<uint8_t*>(dst), offsets);
-  MOLE_LAUNCH_OK();
+  if (int rc = launch_early(align_rows_kernel, grid, 256, 0, st, static_cast<const uint8_t*>(*p), rows, cols * elem,
+                            *ld * elem, static_cast<uint8_t*>(dst), offsets))
+    return rc;
   *p = dst;
   return MOLE_OK;
 }

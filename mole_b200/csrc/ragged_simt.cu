@@ -230,6 +230,7 @@ template <int T, bool KN, bool WIDE>
 __global__ void __launch_bounds__(Tile<T>::kThreads, T == 128 ? 2 : 4)
 ragged_rows_kernel(const RaggedRows a) {
   __shared__ RaggedSpans sp;
+  after_previous();
   if (threadIdx.x < 32) load_spans(sp, a.offsets, a.E, (int)a.R, T == 128 ? 7 : 6);
   __syncthreads();
   const int tile = blockIdx.x;
@@ -285,6 +286,7 @@ template <int T, bool WIDE>
 __global__ void __launch_bounds__(Tile<T>::kThreads, T == 128 ? 2 : 4)
 ragged_wgrad_kernel(const RaggedWgrad a) {
   const int e = blockIdx.z / a.split, part = blockIdx.z % a.split, q0 = blockIdx.x * T, p0 = blockIdx.y * T;
+  after_previous();
   int first, end;
   expert_rows(a.offsets, a.E, (int)a.R, e, first, end);
   const int all = end - first;
@@ -336,7 +338,8 @@ int ragged_wgrad_split(bool tensor, const RaggedWgrad& a) {
 
 // out[i] = part[0][i] + part[1][i] + ...
 template <typename TO>
-__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ part, int split, int64_t n, TO* __restrict__ out) {
+__global__ void __launch_bounds__(256) join_kernel(const float* part, int split, int64_t n, TO* __restrict__ out) {
+  after_previous();
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     float v = part[i];
     for (int s = 1; s < split; ++s) v += part[(int64_t)s * n + i];
@@ -346,10 +349,9 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
 int ragged_join(int out_dtype, const float* part, int split, int64_t n, void* out, cudaStream_t st) {
   int64_t blocks = (n + 255) / 256;
   if (blocks > (int64_t)sm_count() * 8) blocks = (int64_t)sm_count() * 8;
-  if (out_dtype == MOLE_F32) join_kernel<<<(unsigned)blocks, 256, 0, st>>>(part, split, n, static_cast<float*>(out));
-  else join_kernel<<<(unsigned)blocks, 256, 0, st>>>(part, split, n, static_cast<__nv_bfloat16*>(out));
-  MOLE_LAUNCH_OK();
-  return MOLE_OK;
+  const dim3 grid((unsigned)blocks);
+  if (out_dtype == MOLE_F32) return launch_early(join_kernel<float>, grid, 256, 0, st, part, split, n, static_cast<float*>(out));
+  return launch_early(join_kernel<__nv_bfloat16>, grid, 256, 0, st, part, split, n, static_cast<__nv_bfloat16*>(out));
 }
 
 template <bool KN>
@@ -359,12 +361,10 @@ static int launch_rows(const RaggedRows& a, cudaStream_t st) {
   auto grid = [&](int T) {                                                   // every span may end in a partial tile
     return dim3((unsigned)(a.R / T + a.E + 2), (unsigned)((a.N + T - 1) / T), (unsigned)a.split);
   };
-  if (large && wide) ragged_rows_kernel<128, KN, true><<<grid(128), Tile<128>::kThreads, 0, st>>>(a);
-  else if (large) ragged_rows_kernel<128, KN, false><<<grid(128), Tile<128>::kThreads, 0, st>>>(a);
-  else if (wide) ragged_rows_kernel<64, KN, true><<<grid(64), Tile<64>::kThreads, 0, st>>>(a);
-  else ragged_rows_kernel<64, KN, false><<<grid(64), Tile<64>::kThreads, 0, st>>>(a);
-  MOLE_LAUNCH_OK();
-  return MOLE_OK;
+  if (large) return launch_early(wide ? ragged_rows_kernel<128, KN, true> : ragged_rows_kernel<128, KN, false>, grid(128),
+                                 Tile<128>::kThreads, 0, st, a);
+  return launch_early(wide ? ragged_rows_kernel<64, KN, true> : ragged_rows_kernel<64, KN, false>, grid(64),
+                      Tile<64>::kThreads, 0, st, a);
 }
 
 int ragged_rows_simt(const RaggedRows& a, cudaStream_t st) {
@@ -374,13 +374,12 @@ int ragged_rows_simt(const RaggedRows& a, cudaStream_t st) {
 int ragged_wgrad_simt(const RaggedWgrad& a, cudaStream_t st) {
   const bool wide = wide_rows(a.a, a.P) && wide_rows(a.b, a.Q);
   auto grid = [&](int T) { return dim3((unsigned)((a.Q + T - 1) / T), (unsigned)((a.P + T - 1) / T), (unsigned)(a.E * a.split)); };
-  const dim3 g = grid(128);
   const bool large = wgrad_tile(a) == 128;
-  if (large && wide) ragged_wgrad_kernel<128, true><<<g, Tile<128>::kThreads, 0, st>>>(a);
-  else if (large) ragged_wgrad_kernel<128, false><<<g, Tile<128>::kThreads, 0, st>>>(a);
-  else if (wide) ragged_wgrad_kernel<64, true><<<grid(64), Tile<64>::kThreads, 0, st>>>(a);
-  else ragged_wgrad_kernel<64, false><<<grid(64), Tile<64>::kThreads, 0, st>>>(a);
-  MOLE_LAUNCH_OK();
+  if (int rc = large ? launch_early(wide ? ragged_wgrad_kernel<128, true> : ragged_wgrad_kernel<128, false>, grid(128),
+                                    Tile<128>::kThreads, 0, st, a)
+                     : launch_early(wide ? ragged_wgrad_kernel<64, true> : ragged_wgrad_kernel<64, false>, grid(64),
+                                    Tile<64>::kThreads, 0, st, a))
+    return rc;
   return a.split > 1 ? ragged_join(MOLE_F32, a.part, a.split, (int64_t)a.E * a.P * a.Q, a.out, st) : MOLE_OK;
 }
 
