@@ -11,8 +11,8 @@ namespace mole {
 // quotient t is taken as x * (1 / scale), which is off by less than 2^-23 of 127; where that leaves
 // doubt about the nearest integer (1 value in 10^4), the sign of x - (n + 1/2) scale decides, which
 // one fused multiply-add gives exactly.  (A call: inlined 64 times, the kernel misses in the instruction
-// cache.)  Bound by instructions, not by HBM's 3 bytes an element: 32768 x 2048 of bf16 in 53 us (3.8 TB/s;
-// 76 with a division each).
+// cache.)  Bound by instructions, not by HBM's 3 bytes an element: 32768 x 2048 of bf16 in 47 us (4.3 TB/s;
+// half as much again with a division each).
 __device__ __noinline__ int quantize_one(float x, float scale, float inv) {
   const float t = x * inv;
   float r = rintf(t);
@@ -26,9 +26,10 @@ __device__ __noinline__ int quantize_one(float x, float scale, float inv) {
 
 // One row per group of G threads (a warp or a block).  HELD: the row fits the group's registers (eight
 // 16-byte vectors a thread), is read once and waits there for its scale; otherwise it is read twice.
-// V = 1: rows that 16-byte loads cannot address.
+// V = 1: rows that 16-byte loads cannot address.  Four blocks an SM (64 registers): 32768 x 2048 in 47 us; with
+// three, as many as registers allow unasked, 53; with five, which spill, 52.
 template <typename T, int V, int G, bool HELD>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, HELD ? 4 : 1)
 quantize_rows_kernel(const T* x, int64_t R, int K, int8_t* __restrict__ q, float* __restrict__ scale) {
   constexpr int kHeld = 8;
   __shared__ uint32_t tops[8];
