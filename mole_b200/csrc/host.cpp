@@ -106,6 +106,12 @@ at::Tensor output(const at::Tensor* given, const at::Tensor& like, const at::Ten
   TORCH_CHECK_VALUE(!overlap(*given, like) && !overlap(*given, other), "out overlaps an operand");
   return *given;
 }
+// The kernels write through addresses, which autograd does not see: a tensor that a call has written counts
+// its version up, as after an operation of torch in place, so that a backward which still needs what it
+// held before is told (inference tensors have no version)
+void wrote(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 const at::Tensor* maybe(PyObject* o) { return o == Py_None ? nullptr : &tensor_of(o, "out"); }
 
 at::Tensor rows_product(const at::Tensor& x, const at::Tensor& w, const at::Tensor& o, bool kn, const at::Tensor* given) {
@@ -127,6 +133,7 @@ at::Tensor rows_product(const at::Tensor& x, const at::Tensor& w, const at::Tens
   check_status(grouped_mm_(x.data_ptr(), w.data_ptr(), static_cast<const int32_t*>(o.data_ptr()), R, narrow(N), narrow(K),
                            narrow(E), kn, dt, out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes,
                            c10::cuda::getCurrentCUDAStream().stream()));
+  if (given) wrote(out);
   return out;
 }
 
@@ -147,6 +154,7 @@ at::Tensor weight_gradient(const at::Tensor& a, const at::Tensor& b, const at::T
   check_status(grouped_mm_wgrad_(a.data_ptr(), b.data_ptr(), static_cast<const int32_t*>(o.data_ptr()), R, narrow(P), narrow(Q),
                                  narrow(E), dt, out.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes,
                                  c10::cuda::getCurrentCUDAStream().stream()));
+  if (given) wrote(out);
   return out;
 }
 
@@ -250,7 +258,8 @@ PyObject* py_mm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check_with(w, q);
     check_with(ws, q);
     c10::cuda::OptionalCUDAGuard guard(q.device());
-    at::Tensor out = output(maybe(a[6]), q, w, {R, N}, dtype), scratch;
+    const at::Tensor* given = maybe(a[6]);
+    at::Tensor out = output(given, q, w, {R, N}, dtype), scratch;
     int64_t bytes = 0;
     check_status(grouped_mm_workspace_bytes_(q.data_ptr(), w.data_ptr(), R, narrow(N), narrow(K), narrow(E), 0, 1, &bytes));
     if (bytes) scratch = bytes_like(q, bytes);
@@ -258,6 +267,7 @@ PyObject* py_mm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                 static_cast<const float*>(ws.data_ptr()), offsets, R, narrow(N), narrow(K), narrow(E),
                                 dtype == at::kFloat ? MOLE_F32 : MOLE_BF16, out.data_ptr(),
                                 bytes ? scratch.data_ptr() : nullptr, bytes, c10::cuda::getCurrentCUDAStream().stream()));
+    if (given) wrote(out);
     return THPVariable_Wrap(out);
   });
 }
@@ -334,6 +344,8 @@ PyObject* py_adam_multi(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check_status(adam_multi_(table.data(), (int32_t)count, dt, narrow8 ? 8 : 32, b1, b2,
                              t > INT32_MAX ? INT32_MAX : t < 0 ? 0 : (int32_t)t, lr, wd, eps, PyObject_IsTrue(a[12]) == 1,
                              (uint32_t)seed, c10::cuda::getCurrentCUDAStream().stream()));
+    for (const Items* list : {&p, &m, &v, &ms, &vs})
+      for (Py_ssize_t i = 0; i < list->size(); ++i) wrote(list->at(i));
     Py_RETURN_NONE;
   });
 }
