@@ -163,7 +163,8 @@ at::Tensor weight_gradient(const at::Tensor& a, const at::Tensor& b, const at::T
 struct GroupedMM : torch::autograd::Function<GroupedMM> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w,
                             const at::Tensor& offsets, bool kn) {
-    ctx->save_for_backward({x, w, offsets});
+    // each gradient takes the other operand; one that no gradient takes is not held, and may be overwritten
+    ctx->save_for_backward({w.requires_grad() ? x : at::Tensor(), x.requires_grad() ? w : at::Tensor(), offsets});
     ctx->saved_data["kn"] = kn;
     return rows_product(x, w, offsets, kn, nullptr);
   }
@@ -171,8 +172,7 @@ struct GroupedMM : torch::autograd::Function<GroupedMM> {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &w = saved[1], &offsets = saved[2];
     const bool kn = ctx->saved_data["kn"].toBool();
-    TORCH_CHECK(!(at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || grads[0].requires_grad())),
-                "grouped_mm can be differentiated once only");
+    TORCH_CHECK(!at::GradMode::is_enabled(), "grouped_mm can be differentiated once only");
     const at::Tensor dy = grads[0].contiguous();
     at::Tensor dx, dw;
     if (ctx->needs_input_grad(0)) dx = rows_product(dy, w, offsets, !kn, nullptr);

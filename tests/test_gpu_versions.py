@@ -80,3 +80,23 @@ def test_inference_tensors_are_written_too():
     with torch.inference_mode():
         DeviceAdam([q], lr=0.5).step()
     assert (q < 1).all()
+
+
+def test_an_operand_that_no_gradient_takes_may_be_overwritten():
+    """As in torch's own products: dw takes x, dx takes w."""
+    import mole_b200
+    o, x, w = offs([4, 6]), rnd(10, 16), rnd(2, 8, 16, seed=1)
+    for one, other in ((0, 1), (1, 0)):
+        t = [x.clone(), w.clone()]
+        t[one].requires_grad_()
+        y = mole_b200.grouped_mm(*t, o)
+        (want,) = torch.autograd.grad(y.sum(), t[one], retain_graph=True)
+        with torch.no_grad():
+            t[one].mul_(2)
+        (got,) = torch.autograd.grad(y.sum(), t[one], retain_graph=True)
+        assert torch.equal(got, want)
+        with pytest.raises(RuntimeError, match="once only"):
+            torch.autograd.grad(y.sum(), t[one], create_graph=True)
+        t[other].mul_(2)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
