@@ -59,12 +59,19 @@ int mole_device_fault(void* stream, int32_t* fault);
 /* the same check without a host wait, for a training loop: mole_device_fault_poll enqueues a copy
  * of the fault word (of the current device) into pinned host memory behind the work already on
  * `stream`; mole_device_fault_peek returns the value of the last such copy that has landed (0
- * before the first).  MOLECore polls at the end of every backward and peeks at the start of the
+ * before the first), or what a kernel has reported by itself: those of mole_grouped_mm*,
+ * mole_adam_multi and mole_peer_barrier store their code into pinned host memory too, and
+ * mole_grouped_mm*, mole_quantize_rows and mole_adam_multi return MOLE_ERR_DEVICE without launching
+ * anything while a code that has reached the host is not cleared by mole_device_fault.  (They cannot
+ * refuse the call whose own wait runs out: who hands its results on without another call synchronises
+ * and peeks.)  MOLECore polls at the end of every backward and peeks at the start of the
  * next forward.  On a stream that is being captured into a CUDA graph the poll does nothing
  * (its event would become part of the graph): poll behind a replay.  The reference has no
  * counterpart: its device code cannot time out. */
 int mole_device_fault_poll(void* stream);
 int mole_device_fault_peek(int32_t* fault);
+/* what kind of kernel leaves this code, for messages (never null) */
+const char* mole_device_fault_origin(int32_t code);
 
 /* kernels this library has launched in this process (the benchmark reports it) */
 int mole_launch_count(int64_t* n);

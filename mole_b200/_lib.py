@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 from pathlib import Path
+from typing import Optional
 
 _HERE = Path(__file__).resolve().parent
 # MOLE_B200_LIB points at another build of the same library (kernel A/B comparisons)
@@ -48,6 +49,7 @@ SIGNATURES = {
     "mole_device_fault": (C.c_int, [_p, _pi32]),
     "mole_device_fault_poll": (C.c_int, [_p]),
     "mole_device_fault_peek": (C.c_int, [_pi32]),
+    "mole_device_fault_origin": (C.c_char_p, [_i32]),
     "mole_launch_count": (C.c_int, [_pi64]),
     "mole_profile_gemm": (C.c_int, [_i32]),
     "mole_profile_read": (C.c_int, [C.POINTER(C.c_float), _pi32, _i32, _pi32]),
@@ -145,9 +147,10 @@ def _load() -> C.CDLL:
 lib = _load()
 
 
-def check(status: int) -> None:
+def check(status: int, message: Optional[str] = None) -> None:
+    """``message``: where the thread that got the status is not the one that raises it."""
     if status != 0:
-        raise MoleError(status, lib.mole_last_error_string().decode(errors="replace"))
+        raise MoleError(status, lib.mole_last_error_string().decode(errors="replace") if message is None else message)
 
 
 def capacity_stride(capacity: int) -> int:

@@ -626,13 +626,13 @@ class MOLECore:
     def _check_fault(self) -> None:
         """Raises if a kernel of an earlier step recorded that one of its bounded waits ran out
         (that step's activations and gradients are not to be trusted).  Reads a host copy that
-        ``_poll_fault`` requested behind the previous backward: no device synchronisation."""
+        was requested behind the previous backward: no device synchronisation."""
         if torch.cuda.is_current_stream_capturing():
             return          # no event queries while a CUDA graph is being captured (Ugraph polls behind replays)
         code = ops.device_fault_peek()
         if code:
             raise RuntimeError(
-                f"a grouped-GEMM kernel gave up on a bounded wait (fault code {code}): the results "
+                f"{ops.device_fault_origin(code)} gave up on a bounded wait (fault code {code}): the results "
                 "of that step are invalid")
 
     def _desc(self, M, F, n_src, Cs, rec: Record, n_slots, accumulate=False, n_grad_slots=0,

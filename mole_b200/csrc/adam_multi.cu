@@ -616,6 +616,7 @@ adam_multi_kernel(const __grid_constant__ AdamTable<CAP> table, const __grid_con
   if (abort_s) {                                    // loads under way get time to land
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 20000000ull) __nanosleep(1000);
+    if (threadIdx.x == 0) report_fault(a.fault);
     return;
   }
   // what the whole blocks' form left over, now that its stores are done
@@ -703,6 +704,7 @@ extern "C" int mole_adam_multi(const mole_adam_tensor* tensors, int32_t n_tensor
                      ((reinterpret_cast<uintptr_t>(x.m_scale) | reinterpret_cast<uintptr_t>(x.v_scale)) & 3) == 0,
                  "tensor %d: a pointer is not aligned to its element", i);
   }
+  if (int rc = check_no_fault()) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
   MOLE_CUDA_OK(cudaStreamIsCapturing(st, &cap));

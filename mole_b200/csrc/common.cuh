@@ -84,6 +84,17 @@ int launch_gate_wgrad_mma(const float* dlogits, const void* x, int64_t T, int M,
 
 // device-side fault word: kernels with bounded waits record where they gave up
 int32_t* device_fault_word();   // of the current device; allocated at its first use (256 bytes), zeroed
+// MOLE_ERR_DEVICE while a fault that has reached the host is not cleared (mole_device_fault); one read of
+// pinned memory, no wait
+int check_no_fault();
+// What is in the fault word, to the host as well: by one thread of a kernel whose wait has run out, so that
+// the calls after it know without a poll.  word + 2 holds the address of the pinned copy.
+__device__ __forceinline__ void report_fault(const int32_t* word) {
+  volatile int32_t* host = *reinterpret_cast<int32_t* const volatile*>(word + 2);
+  if (host == nullptr) return;
+  *host = *static_cast<const volatile int32_t*>(word);
+  __threadfence_system();
+}
 
 // Per-device host state.  cudaFuncSetAttribute, occupancy figures and the SM count belong to a
 // device, not to the process: a process that drives several GPUs needs them once per device.

@@ -11,6 +11,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -63,6 +64,13 @@ void check_status(int rc) {
 }
 at::Tensor bytes_like(const at::Tensor& t, int64_t n) { return at::empty({n}, t.options().dtype(at::kByte)); }
 
+// Sets the Python exception of a status; holds the interpreter's lock
+void set_exception(const StatusError& e) {
+  PyObject* r = PyObject_CallFunction(check_, "is", e.status, e.what());
+  Py_XDECREF(r);
+  if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+}
+
 // No C++ exception passes into the interpreter
 template <typename F>
 PyObject* guarded(F&& f) {
@@ -70,9 +78,7 @@ PyObject* guarded(F&& f) {
     return f();
   } catch (const PyRaised&) {
   } catch (const StatusError& e) {
-    PyObject* r = PyObject_CallFunction(check_, "i", e.status);
-    Py_XDECREF(r);
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+    set_exception(e);
   } catch (const c10::TypeError& e) {
     PyErr_SetString(PyExc_TypeError, e.what_without_backtrace());
   } catch (const c10::ValueError& e) {
@@ -175,8 +181,17 @@ struct GroupedMM : torch::autograd::Function<GroupedMM> {
     TORCH_CHECK(!at::GradMode::is_enabled(), "grouped_mm can be differentiated once only");
     const at::Tensor dy = grads[0].contiguous();
     at::Tensor dx, dw;
-    if (ctx->needs_input_grad(0)) dx = rows_product(dy, w, offsets, !kn, nullptr);
-    if (ctx->needs_input_grad(1)) dw = kn ? weight_gradient(x, dy, offsets, nullptr) : weight_gradient(dy, x, offsets, nullptr);
+    try {
+      if (ctx->needs_input_grad(0)) dx = rows_product(dy, w, offsets, !kn, nullptr);
+      if (ctx->needs_input_grad(1)) dw = kn ? weight_gradient(x, dy, offsets, nullptr) : weight_gradient(dy, x, offsets, nullptr);
+    } catch (const StatusError& e) {     // on a thread of the engine: the exception of its kind travels with its error
+      const PyGILState_STATE lock = PyGILState_Ensure();
+      set_exception(e);
+      python_error raised;
+      raised.persist();
+      PyGILState_Release(lock);
+      throw raised;
+    }
     return {dx, dw, at::Tensor(), at::Tensor()};
   }
 };

@@ -261,6 +261,7 @@ extern "C" int mole_grouped_mm(const void* x, const void* w, const int32_t* offs
   RaggedRows a{};
   a.x = x; a.w = w; a.offsets = offsets; a.out = out;
   a.R = R; a.N = N; a.K = K; a.E = E; a.kn = w_kn != 0;
+  if (int rc = check_no_fault()) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (ragged_rows_few_takes(a)) return ragged_rows_few(dtype, a, st);
   Aligner ws{static_cast<uint8_t*>(workspace), workspace_bytes, 0, false};
@@ -303,6 +304,7 @@ extern "C" int mole_grouped_mm_wgrad(const void* a, const void* b, const int32_t
   RaggedWgrad g{};
   g.a = a; g.b = b; g.offsets = offsets; g.out = out;
   g.R = R; g.P = P; g.Q = Q; g.E = E;
+  if (int rc = check_no_fault()) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   Aligner ws{static_cast<uint8_t*>(workspace), workspace_bytes, 0, false};
   g.split = ragged_wgrad_split(dtype == MOLE_BF16, g);
@@ -344,6 +346,7 @@ extern "C" int mole_quantize_rows(const void* x, int64_t R, int32_t K, int32_t d
   if (R == 0) return MOLE_OK;
   MOLE_REQUIRE(x && q && scale, "null pointer argument");
   MOLE_REQUIRE(aligned_to(x, dtype == MOLE_F32 ? 4 : 2) && aligned_to(scale, 4), "a pointer is not aligned to its element");
+  if (int rc = check_no_fault()) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == MOLE_F32 ? launch_quantize<float>(x, R, K, q, scale, st)
                            : launch_quantize<__nv_bfloat16>(x, R, K, q, scale, st);
@@ -364,6 +367,7 @@ extern "C" int mole_grouped_mm_i8(const void* q, const float* q_scale, const voi
   RaggedRows a{};
   a.x = q; a.w = w; a.offsets = offsets; a.x_scale = q_scale; a.w_scale = w_scale; a.out = out;
   a.R = R; a.N = N; a.K = K; a.E = E;
+  if (int rc = check_no_fault()) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (ragged_rows_few_takes(a)) return ragged_rows_few_i8(out_dtype, a, st);
   if (int rc = align_rows(a, 1, Aligner{static_cast<uint8_t*>(workspace), workspace_bytes, 0, false}, nullptr, st)) return rc;

@@ -26,7 +26,7 @@
 // 0.63 ms, 1.7 POP/s.
 //
 // Every wait is bounded: a wait that runs out leaves a code in the fault word, the CTA's other roles
-// stop at their next wait, copies in flight get time to land, the TMEM is freed.
+// stop at their next wait, copies in flight get time to land, the host is told, the TMEM is freed.
 #include <type_traits>
 
 #include "ragged.cuh"
@@ -451,7 +451,10 @@ ragged_rows_tc_kernel(const __grid_constant__ RowsMaps maps, const __grid_consta
   }
 
   __syncwarp();
-  if (*abort_flag) settle();
+  if (*abort_flag) {
+    settle();
+    if (threadIdx.x == 0) report_fault(p.fault);
+  }
   __syncwarp();
   tcgen05_fence_before();
   cluster_meet();              // nobody leaves while the peer may still touch its shared memory
@@ -761,7 +764,10 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   }
 
   __syncwarp();
-  if (*abort_flag) settle();
+  if (*abort_flag) {
+    settle();
+    if (threadIdx.x == 0) report_fault(p.fault);
+  }
   __syncwarp();
   tcgen05_fence_before();
   cluster_meet();

@@ -24,8 +24,9 @@ char* last_error_buffer() {
 
 // One fault word per device (256 bytes of device memory, allocated at the device's first use).
 struct FaultSlot {
-  int32_t* word = nullptr;        // device
-  int32_t* host = nullptr;        // pinned: where mole_device_fault_poll copies the word
+  int32_t* word = nullptr;        // device: the word; word + 2: the address of host + 2
+  // pinned: [0] the last poll's copy that was seen to land, [1] where polls store, [2] where report_fault does
+  std::atomic<int32_t*> host{nullptr};
   cudaEvent_t polled = nullptr;   // recorded behind the last poll's copy
   bool poll_pending = false;
 };
@@ -38,8 +39,13 @@ static FaultSlot* fault_slot() {
   if (!f.word) {
     if (cudaMalloc(&f.word, 256) != cudaSuccess) { f.word = nullptr; return nullptr; }
     cudaMemset(f.word, 0, 256);
-    if (cudaMallocHost(&f.host, 64) != cudaSuccess) f.host = nullptr;
-    else *f.host = 0;
+    int32_t* host = nullptr;
+    if (cudaMallocHost(&host, 64) == cudaSuccess) {
+      std::memset(host, 0, 64);
+      int32_t* direct = host + 2;
+      cudaMemcpy(f.word + 2, &direct, sizeof(direct), cudaMemcpyHostToDevice);
+      f.host.store(host, std::memory_order_release);
+    }
     if (cudaEventCreateWithFlags(&f.polled, cudaEventDisableTiming) != cudaSuccess) f.polled = nullptr;
   }
   return &f;
@@ -47,6 +53,19 @@ static FaultSlot* fault_slot() {
 int32_t* device_fault_word() {
   FaultSlot* f = fault_slot();
   return f ? f->word : nullptr;
+}
+
+// code of the current device's fault as far as the host knows it; 0: none
+static int32_t known_fault() {
+  const volatile int32_t* h = g_fault[current_device()].host.load(std::memory_order_acquire);
+  if (h == nullptr) return 0;
+  return h[2] != 0 ? h[2] : h[1] != 0 ? h[1] : h[0];
+}
+int check_no_fault() {
+  const int32_t code = known_fault();
+  if (code == 0) return MOLE_OK;
+  return fail(MOLE_ERR_DEVICE, "%s gave up on a bounded wait (fault code %d): what was computed since is not to be used "
+              "(mole_device_fault reads and clears the code)", mole_device_fault_origin(code), code);
 }
 
 int sm_count() {
@@ -122,7 +141,17 @@ extern "C" int mole_device_fault(void* stream, int32_t* fault) {
   MOLE_CUDA_OK(cudaMemcpyAsync(fault, w, 4, cudaMemcpyDeviceToHost, st));
   MOLE_CUDA_OK(cudaStreamSynchronize(st));
   if (*fault != 0) MOLE_CUDA_OK(cudaMemsetAsync(w, 0, 4, st));
+  if (int32_t* h = g_fault[current_device()].host.load(std::memory_order_acquire)) h[0] = h[1] = h[2] = 0;
   return MOLE_OK;
+}
+extern "C" const char* mole_device_fault_origin(int32_t code) {
+  switch (code / 10) {
+    case 0: case 1: case 2: case 3: return code > 0 ? "a grouped-GEMM kernel of the expert FFN" : "no kernel";
+    case 6: return "a product over packed rows";
+    case 7: return "a weight gradient over packed rows";
+    case 8: return "an Adam step over many tensors";
+    default: return code >= 40 && code < 40 + kMaxPeers ? "a barrier that a rank did not reach" : "a kernel";
+  }
 }
 // The same check without a host wait: poll enqueues a copy of the word into pinned host memory
 // behind the work already on `stream`; peek returns the last copy that has landed.
@@ -135,7 +164,8 @@ __global__ void fault_word_to_host_kernel(const int32_t* __restrict__ word, vola
 
 extern "C" int mole_device_fault_poll(void* stream) {
   FaultSlot* f = fault_slot();
-  if (!f || !f->host || !f->polled) return fail(MOLE_ERR_CUDA, "fault word not allocated");
+  int32_t* host = f ? f->host.load(std::memory_order_acquire) : nullptr;
+  if (!host || !f->polled) return fail(MOLE_ERR_CUDA, "fault word not allocated");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   // A stream that is being captured into a CUDA graph takes no poll: the event of the copy would
   // become part of the graph and could no longer be queried.  Whoever replays the graph polls
@@ -146,7 +176,7 @@ extern "C" int mole_device_fault_poll(void* stream) {
     cudaGetLastError();           // the previous poll's copy is still in flight: keep that one
     return MOLE_OK;
   }
-  fault_word_to_host_kernel<<<1, 1, 0, st>>>(f->word, f->host + 1);
+  fault_word_to_host_kernel<<<1, 1, 0, st>>>(f->word, host + 1);
   MOLE_LAUNCH_OK();
   MOLE_CUDA_OK(cudaEventRecord(f->polled, st));
   f->poll_pending = true;
@@ -155,14 +185,16 @@ extern "C" int mole_device_fault_poll(void* stream) {
 extern "C" int mole_device_fault_peek(int32_t* fault) {
   MOLE_REQUIRE(fault != nullptr, "fault is null");
   FaultSlot* f = fault_slot();
-  if (!f || !f->host || !f->polled) return fail(MOLE_ERR_CUDA, "fault word not allocated");
+  int32_t* host = f ? f->host.load(std::memory_order_acquire) : nullptr;
+  if (!host || !f->polled) return fail(MOLE_ERR_CUDA, "fault word not allocated");
   if (f->poll_pending && cudaEventQuery(f->polled) == cudaSuccess) {
-    f->host[0] = f->host[1];
+    host[0] = static_cast<volatile int32_t*>(host)[1];
     f->poll_pending = false;
   } else {
     cudaGetLastError();
   }
-  *fault = f->host[0];
+  const int32_t direct = static_cast<volatile int32_t*>(host)[2];
+  *fault = direct != 0 ? direct : host[0];
   return MOLE_OK;
 }
 
@@ -445,6 +477,7 @@ __global__ void peer_barrier_kernel(const __grid_constant__ PeerFlags f, int wor
       asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
       if (t - t0 > limit_ns) {
         atomicCAS(fault, 0, 40 + q);
+        report_fault(fault);
         return;
       }
     }

@@ -3,7 +3,9 @@
 PyTorch owns device memory and streams; every function here checks shapes, allocates outputs
 with ``torch.empty`` and hands raw pointers to ``libmole_b200.so`` on the current stream.
 None of them has a PyTorch fallback.  The products over packed rows and the Adam step over many tensors
-do the same in ``_host.so``, on the current stream of their tensors' device.
+do the same in ``_host.so``, on the current stream of their tensors' device; they raise ``MoleError``
+(``MOLE_ERR_DEVICE``) once the host knows that a kernel gave up on a bounded wait, until ``device_fault()``
+has read and cleared its code.
 """
 from __future__ import annotations
 
@@ -373,14 +375,20 @@ def device_fault_poll() -> None:
 
 
 def device_fault_peek() -> int:
-    """Value of the last polled copy that has landed (0 before the first)."""
+    """Value of the last polled copy that has landed (0 before the first), or what a kernel of the products
+    over packed rows, ``adam_multi`` or a barrier has reported by itself."""
     f = C.c_int32()
     check(lib.mole_device_fault_peek(C.byref(f)))
     return f.value
 
 
+def device_fault_origin(code: int) -> str:
+    """What kind of kernel leaves this code."""
+    return lib.mole_device_fault_origin(code).decode()
+
+
 def device_fault() -> int:
-    """Code left by a kernel whose bounded wait ran out (0 = none); synchronises the stream."""
+    """Code left by a kernel whose bounded wait ran out (0 = none), which it clears; synchronises the stream."""
     f = C.c_int32()
     check(lib.mole_device_fault(_stream(), C.byref(f)))
     return f.value

@@ -51,5 +51,6 @@ class GraphedStep:
             ops.device_fault_poll()
             code = ops.device_fault_peek()
             if code:
-                raise RuntimeError(f"a kernel of a replayed step gave up on a bounded wait (fault code {code})")
+                raise RuntimeError(f"{ops.device_fault_origin(code)} gave up on a bounded wait in a replayed step "
+                                   f"(fault code {code})")
         return self.outputs
