@@ -25,15 +25,17 @@ def unpack_moment(codes: torch.Tensor, scale: torch.Tensor, square: bool) -> tor
 
 
 def pack_moment(values: torch.Tensor, square: bool) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Codes and scales of fp32 values, rounded to nearest: for states that come from elsewhere."""
+    """Codes and scales of fp32 values, rounded to nearest: for states that come from elsewhere.  As in a
+    step, a value that is NaN stays so, one that is infinite becomes its block's largest code (NaN in a block of
+    zeros), and neither touches its neighbours."""
     flat = values.reshape(-1).float()
     if square:
         flat = flat.sqrt()
     n = flat.numel()
     blocks = torch.nn.functional.pad(flat, (0, -n % ops.ADAM_BLOCK)).view(-1, ops.ADAM_BLOCK)
-    top = blocks.abs().amax(1, keepdim=True)
+    top = torch.where(blocks.isfinite(), blocks.abs(), 0.0).amax(1, keepdim=True)
     live = top >= 2.0 ** -100
-    y = torch.where(live, blocks / torch.where(live, top, 1.0) * _E4M3_MAX, 0.0)
+    y = torch.where(live, blocks / torch.where(live, top, 1.0) * _E4M3_MAX, blocks * 0.0)
     if square:      # a second moment that is not zero is never held as zero
         y = torch.where((blocks > 0) & live, y.clamp(min=2.0 ** -9), y)
     codes = y.clamp_(-_E4M3_MAX, _E4M3_MAX).flatten()[:n].to(torch.float8_e4m3fn).view(values.shape)
