@@ -316,7 +316,8 @@ int mole_ffn_bwd_peer(const mole_ffn_desc* desc, const int32_t* counts,
  * clamped on the device to a rising sequence in [0, R].  Any width and element-aligned pointers are
  * taken.  The workspace (its size from the _workspace_bytes calls; null will do for 0) holds copies of
  * bf16 and 8-bit operands whose rows do not start on 16 bytes, and partial results where a product
- * has too few tiles for the SMs and its reduction is cut into parts; 0 for up to 16 rows.  All sums are
+ * has too few tiles for the SMs and its reduction is cut into parts; 0 for mole_grouped_mm and
+ * mole_grouped_mm_i8 of up to 16 rows (the weight gradient copies at any number of rows).  All sums are
  * held in 32 bits, parts are joined in their order, and a result is rounded once.
  * The reference computes the same products inside bffn_fwd / bffn_bwd over capacity-padded rows
  * (MOLE/cpp/core.cpp:350-353, 388-412).
@@ -473,8 +474,9 @@ int mole_adam_update(void* p, void* m, void* v, const void* g, const void* g_ext
  * (seed, t, index in the list, element) alone.  A block whose largest moment is below 2^-100 is held
  * as zeros; a moment that is NaN stays so and one that is infinite is held as its block's largest
  * code (as NaN in a block of zeros), neither touching its neighbours.  t, lr and the rest as in mole_adam_update.  The list is a
- * host array, read before the call returns.  Pointers need the alignment of their elements only
- * (16 bytes, 8 for 8-bit moments, for the wide accesses).  t and lr are taken by value, so a stream
+ * host array, read before the call returns.  Pointers need the alignment of their elements only; a
+ * tensor whose p, g, m and v all start on 16 bytes travels by bulk copies, another one by loads of single
+ * elements, several times as slow.  t and lr are taken by value, so a stream
  * under capture is refused (MOLE_ERR_STATE).  A tensor may appear once per call. */
 typedef struct {
   void* p;
