@@ -477,7 +477,8 @@ int mole_adam_update(void* p, void* m, void* v, const void* g, const void* g_ext
  * host array, read before the call returns.  Pointers need the alignment of their elements only; a
  * tensor whose p, g, m and v all start on 16 bytes travels by bulk copies, another one by loads of single
  * elements, several times as slow.  t and lr are taken by value, so a stream
- * under capture is refused (MOLE_ERR_STATE).  A tensor may appear once per call. */
+ * under capture is refused (MOLE_ERR_STATE).  No two of the arrays that a call writes (p, m, v and the scales of all its
+ * tensors) may overlap, nor a gradient what another tensor writes. */
 typedef struct {
   void* p;
   const void* g;
