@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <stdexcept>
 #include <vector>
 
@@ -104,12 +105,15 @@ bool overlap(const at::Tensor& a, const at::Tensor& b) {
   const char* y = static_cast<const char*>(b.data_ptr());
   return x < y + b.nbytes() && y < x + a.nbytes();
 }
-at::Tensor output(const at::Tensor* given, const at::Tensor& like, const at::Tensor& other, at::IntArrayRef shape,
-                  at::ScalarType dtype) {
+// The given output, or a new one on the device of `like`; `others`: what else the call reads
+at::Tensor output(const at::Tensor* given, const at::Tensor& like, std::initializer_list<const at::Tensor*> others,
+                  at::IntArrayRef shape, at::ScalarType dtype) {
   if (given == nullptr) return at::empty(shape, like.options().dtype(dtype));
   TORCH_CHECK_VALUE(given->sizes() == shape && given->scalar_type() == dtype, "out must be ", dtype, " ", shape);
   check_with(*given, like);
-  TORCH_CHECK_VALUE(!overlap(*given, like) && !overlap(*given, other), "out overlaps an operand");
+  bool clear = !overlap(*given, like);
+  for (const at::Tensor* t : others) clear = clear && (t == nullptr || !overlap(*given, *t));
+  TORCH_CHECK_VALUE(clear, "out overlaps an operand");
   return *given;
 }
 // The kernels write through addresses, which autograd does not see: a tensor that a call has written counts
@@ -131,7 +135,7 @@ at::Tensor rows_product(const at::Tensor& x, const at::Tensor& w, const at::Tens
   check_with(w, x);
   check_with(o, x);
   c10::cuda::OptionalCUDAGuard guard(x.device());
-  at::Tensor out = output(given, x, w, {R, N}, x.scalar_type()), ws;
+  at::Tensor out = output(given, x, {&w, &o}, {R, N}, x.scalar_type()), ws;
   int64_t bytes = 0;
   check_status(grouped_mm_workspace_bytes_(x.data_ptr(), w.data_ptr(), R, narrow(N), narrow(K), narrow(E), kn,
                                            (int32_t)x.element_size(), &bytes));
@@ -153,7 +157,7 @@ at::Tensor weight_gradient(const at::Tensor& a, const at::Tensor& b, const at::T
   check_with(b, a);
   check_with(o, a);
   c10::cuda::OptionalCUDAGuard guard(a.device());
-  at::Tensor out = output(given, a, b, {E, P, Q}, a.scalar_type()), ws;
+  at::Tensor out = output(given, a, {&b, &o}, {E, P, Q}, a.scalar_type()), ws;
   int64_t bytes = 0;
   check_status(grouped_mm_wgrad_workspace_bytes_(a.data_ptr(), b.data_ptr(), R, narrow(P), narrow(Q), narrow(E), dt, &bytes));
   if (bytes) ws = bytes_like(a, bytes);
@@ -251,12 +255,12 @@ PyObject* py_mm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const bool grouped = a[4] != Py_None;
     TORCH_CHECK_VALUE(w.dim() == (grouped ? 3 : 2), grouped ? "grouped_mm_int8 takes w [E, N, K]" : "mm_int8 takes w [N, K]");
     const int64_t E = grouped ? w.size(0) : 1, N = w.size(-2), K = w.size(-1);
+    const at::Tensor* o = grouped ? &tensor_of(a[4], "offsets") : nullptr;
     const int32_t* offsets = nullptr;
     if (grouped) {
-      const at::Tensor& o = tensor_of(a[4], "offsets");
-      check_offsets(o, E);
-      check_with(o, q);
-      offsets = static_cast<const int32_t*>(o.data_ptr());
+      check_offsets(*o, E);
+      check_with(*o, q);
+      offsets = static_cast<const int32_t*>(o->data_ptr());
     }
     TORCH_CHECK_TYPE(q.scalar_type() == at::kChar && w.scalar_type() == at::kChar, "the operands must be int8");
     TORCH_CHECK_VALUE(q.dim() == 2 && q.size(1) == K, "q must be [R, ", K, "]");
@@ -274,7 +278,7 @@ PyObject* py_mm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check_with(ws, q);
     c10::cuda::OptionalCUDAGuard guard(q.device());
     const at::Tensor* given = maybe(a[6]);
-    at::Tensor out = output(given, q, w, {R, N}, dtype), scratch;
+    at::Tensor out = output(given, q, {&w, &qs, &ws, o}, {R, N}, dtype), scratch;
     int64_t bytes = 0;
     check_status(grouped_mm_workspace_bytes_(q.data_ptr(), w.data_ptr(), R, narrow(N), narrow(K), narrow(E), 0, 1, &bytes));
     if (bytes) scratch = bytes_like(q, bytes);
