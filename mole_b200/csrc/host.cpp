@@ -37,6 +37,16 @@ PyObject* out_of_memory_ = nullptr;      // torch.cuda.OutOfMemoryError
 
 struct PyRaised {};                      // a Python exception is set
 
+double number(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw PyRaised();
+  return v;
+}
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw PyRaised();
+  return v == 1;
+}
 const at::Tensor& tensor_of(PyObject* o, const char* what) {
   TORCH_CHECK_TYPE(THPVariable_Check(o), what, " must be a tensor");
   return THPVariable_Unpack(o);
@@ -204,16 +214,16 @@ struct GroupedMM : torch::autograd::Function<GroupedMM> {
 PyObject* py_grouped_mm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     TORCH_CHECK(n == 5, "grouped_mm takes 5 arguments");
-    return THPVariable_Wrap(rows_product(tensor_of(a[0], "x"), tensor_of(a[1], "w"), tensor_of(a[2], "offsets"),
-                                         PyObject_IsTrue(a[3]) == 1, maybe(a[4])));
+    const bool kn = truth(a[3]);
+    return THPVariable_Wrap(rows_product(tensor_of(a[0], "x"), tensor_of(a[1], "w"), tensor_of(a[2], "offsets"), kn, maybe(a[4])));
   });
 }
 // grouped_mm_autograd(x, w, offsets, w_kn)
 PyObject* py_grouped_mm_autograd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     TORCH_CHECK(n == 4, "grouped_mm_autograd takes 4 arguments");
-    return THPVariable_Wrap(GroupedMM::apply(tensor_of(a[0], "x"), tensor_of(a[1], "w"), tensor_of(a[2], "offsets"),
-                                             PyObject_IsTrue(a[3]) == 1));
+    const bool kn = truth(a[3]);
+    return THPVariable_Wrap(GroupedMM::apply(tensor_of(a[0], "x"), tensor_of(a[1], "w"), tensor_of(a[2], "offsets"), kn));
   });
 }
 // grouped_mm_wgrad(a, b, offsets, out)
@@ -303,11 +313,6 @@ struct Items {
   Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(fast); }
   const at::Tensor& at(Py_ssize_t i) const { return tensor_of(PySequence_Fast_GET_ITEM(fast, i), "an item"); }
 };
-double number(PyObject* o) {
-  const double v = PyFloat_AsDouble(o);
-  if (v == -1.0 && PyErr_Occurred()) throw PyRaised();
-  return v;
-}
 // What a call writes, a run of addresses per list (m, v, ...): no two ranges may overlap, or thread blocks would
 // race on them.  Lists mostly come in the order of their addresses, so that this is a merge of sorted runs
 // (a call over 400 tensors takes the host 41 us with 32-bit states, 64 with 8-bit ones; 5 and 18 of it are for
@@ -356,6 +361,7 @@ PyObject* py_adam_multi(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const double t = number(a[6]), lr = number(a[7]), b1 = number(a[8]), b2 = number(a[9]), eps = number(a[10]), wd = number(a[11]);
     const unsigned long long seed = PyLong_AsUnsignedLongLongMask(a[13]);
     if (seed == (unsigned long long)-1 && PyErr_Occurred()) throw PyRaised();
+    const bool adamw = truth(a[12]);
     const Items p(a[0]), g(a[1]), m(a[2]), v(a[3]);
     const Py_ssize_t count = p.size();
     TORCH_CHECK_VALUE(g.size() == count && m.size() == count && v.size() == count,
@@ -407,7 +413,7 @@ PyObject* py_adam_multi(PyObject*, PyObject* const* a, Py_ssize_t n) {
     written.check();
     c10::cuda::OptionalCUDAGuard guard(first.device());
     check_status(adam_multi_(table.data(), (int32_t)count, dt, narrow8 ? 8 : 32, b1, b2,
-                             t > INT32_MAX ? INT32_MAX : t < 0 ? 0 : (int32_t)t, lr, wd, eps, PyObject_IsTrue(a[12]) == 1,
+                             t > INT32_MAX ? INT32_MAX : t < 0 ? 0 : (int32_t)t, lr, wd, eps, adamw,
                              (uint32_t)seed, c10::cuda::getCurrentCUDAStream().stream()));
     for (const at::Tensor* x : written.tensors) wrote(*x);
     Py_RETURN_NONE;
