@@ -7,6 +7,7 @@ the host side of the calls whose checks would take longer in Python than they do
 """
 from __future__ import annotations
 
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -21,6 +22,7 @@ CSRC = HERE / "csrc"
 OUT_DIR = HERE / "lib"
 LIB = OUT_DIR / "libmole_b200.so"
 HOST_LIB = OUT_DIR / "_host.so"          # extension module over torch's tensors (host.cpp)
+HOST_STAMP = OUT_DIR / "_host.built_for"  # the Python and torch that it was built for
 SOURCES = ["route.cu", "dispatch.cu", "gate_mma.cu", "gemm_simt.cu", "gemm_tc.cu", "ffn.cu", "runtime.cu", "adam.cu",
            "adam_multi.cu", "ragged.cu", "ragged_simt.cu", "ragged_tc.cu", "ragged_few.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -38,6 +40,15 @@ def _nccl_include() -> list[str]:
     return ["-I", str(site)] if (site / "nccl.h").exists() else []
 
 
+def host_abi() -> str:
+    """What the extension module has to be built for: this Python and this torch."""
+    try:
+        torch = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:      # a source tree
+        torch = "of a source tree"
+    return f"{sys.implementation.cache_tag}, torch {torch}"
+
+
 def _build_host(nvcc: str) -> None:
     # by way of nvcc, so that the compiler is the one the library is built with: $CXX may be a tool chain
     # whose modules crash under torch
@@ -50,10 +61,13 @@ def _build_host(nvcc: str) -> None:
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError("building _host.so failed")
+    HOST_STAMP.write_text(host_abi())
 
 
 def _stale() -> bool:
     if not LIB.exists() or not HOST_LIB.exists():
+        return True
+    if not HOST_STAMP.exists() or HOST_STAMP.read_text() != host_abi():
         return True
     newest = max(p.stat().st_mtime for p in list(CSRC.iterdir()) + [HERE.parent / "include" / "mole_b200.h"])
     return newest > min(LIB.stat().st_mtime, HOST_LIB.stat().st_mtime)
