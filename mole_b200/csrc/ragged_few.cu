@@ -1,7 +1,8 @@
 // Products over few rows packed by expert (up to 16 in all: decode steps), every type and layout.
 //
-// With that few rows a product is one reading of the weights of the experts that have rows: 2 N K
-// bytes of bf16 per expert, a row's worth of multiply-adds on each, which the CUDA cores keep up with.
+// With that few rows a product is a reading of the weights of the experts that have rows: 2 N K
+// bytes of bf16 per expert, a row's worth of multiply-adds on each, which the CUDA cores keep up with for
+// up to four rows of an expert; every four more read its weights once more.
 // What counts is loads in flight.  The tensor-core kernel gives a decode step one pair of SMs per
 // 256 features (64 pairs at best, and a pipeline to fill); here every warp of every SM streams weights:
 // one token with two of 64 experts of 2048 x 8192 takes 15 us (67 MB at 4.5 TB/s), there 22.
@@ -271,6 +272,21 @@ few_kn_kernel(const RaggedRows a) {
   }
 }
 
+// By all rows together: the host does not know how they fall to the experts.  Measured against the forms
+// for more rows (tensor cores, for fp32 the tiles), in us, three sets of weights in turn; 17 rows take those:
+//   rows                                1         4         8        16       17
+//   bf16, 64 experts of 2048 x 2048   5.3/16   9.8/17    15/18    27/32      31
+//   bf16, the same N-major            8.0/16    16/17    32/17    63/32      31
+//   8 bits, 64 of 2048 x 2048         4.1/11   6.4/11   8.6/12    15/20      20
+//   fp32, 64 of 2048 x 2048           6.6/83   15/81     27/117   47/191    174
+//   bf16, one expert of 8192 x 8192    27/46    39/46    74/46   142/46      46
+//   bf16, the same N-major             54/46    66/46   129/46   257/46      46
+//   8 bits, one of 8192 x 8192         13/25    16/25    28/25    52/25      25
+//   fp32, one of 8192 x 8192          45/155   49/156   95/158  192/162     251
+//   fp32, the same N-major            69/119    82/120  162/122   323/126     230
+// So the rule is right where rows fall to many experts, but for bf16 and N-major weights from five rows on;
+// for one expert it is right up to four rows (not for bf16 and N-major weights) and wrong from eight on (fp32
+// and K-major weights: from sixteen).
 bool ragged_rows_few_takes(const RaggedRows& a) { return a.R <= 16; }
 
 template <typename T, typename TO>

@@ -1,5 +1,6 @@
-// fp32 products over rows packed by expert, on the CUDA cores: they have to be exact to 2^-24, which the
-// tensor cores' input types are not.  Every size and alignment.
+// fp32 products over rows packed by expert, on the CUDA cores: operands of 24 bits, which one term of bf16
+// does not hold (three would; products of split operands on the tensor cores are not tried here).  Every size
+// and alignment.
 //
 // A thread block takes a tile of T x T outputs, a thread 16 x 8 of them in registers (4 x 4 for T = 64);
 // tiles of both operands, 16 deep in the reduction, go through shared memory, the next ones on their way

@@ -19,11 +19,13 @@
 // over them in shared memory, in both operands, before that stage is handed to the tensor cores.
 // There are no padding rows in memory to do without it, and 16 rows are all that is wasted.
 //
-// What bounds them: with every SM at work the board's power (1000 W; the clock falls to 1.0 to 1.4 GHz of
-// 1.97).  64 experts of 256 rows, 2048 x 8192: 0.55, 0.50 and 0.69 ms for the three products back to back
-// (1.0, 1.1 and 0.8 PFLOP/s), 0.48, 0.47 and 0.60 when the board is cool; a batched library product of the
-// same equal batches 0.62, 0.59 and 0.70 back to back.  Integers, 32768 rows of 128 experts, 2048 -> 8192:
-// 0.63 ms, 1.7 POP/s.
+// What bounds them: in a single launch the waits for the ring and, in the weight gradient, for accumulators; in
+// a long run the board's power as well (the clock falls to 1.0 to 1.5 GHz of 1.97).  64 experts of 256 rows,
+// 8192 -> 2048, N-major: 0.45, 0.44 and 0.57 ms for the three products in single launches (1.2, 1.2 and
+// 1.0 PFLOP/s; memory 5.5, 5.6 and 4.4 TB/s), 0.58, 0.58 and 0.71 back to back for seconds; a batched library
+// product of the same equal batches 0.54 (forward) and 0.59 (dw), 0.63 and 0.71.  12 experts of 340 rows,
+// 2048 -> 8192: 0.14, 0.16 and 0.17 ms, the library's 0.12 and 0.15.  Integers, 32768 rows of 128 experts,
+// 2048 -> 8192: 0.49 ms in a single launch, 0.63 back to back (2.3 and 1.75 POP/s).
 //
 // Every wait is bounded: a wait that runs out leaves a code in the fault word, the CTA's other roles
 // stop at their next wait, copies in flight get time to land, the host is told, the TMEM is freed.
