@@ -453,13 +453,11 @@ ragged_rows_tc_kernel(const __grid_constant__ RowsMaps maps, const __grid_consta
   }
 
   __syncwarp();
-  if (*abort_flag) {
-    settle();
-    if (threadIdx.x == 0) report_fault(p.fault);
-  }
+  if (*abort_flag) settle();
   __syncwarp();
   tcgen05_fence_before();
   cluster_meet();              // nobody leaves while the peer may still touch its shared memory
+  if (threadIdx.x == 0 && *abort_flag) report_fault(p.fault);      // whichever warp's wait it was
   if (warp == 1) {
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
@@ -766,13 +764,11 @@ ragged_wgrad_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_c
   }
 
   __syncwarp();
-  if (*abort_flag) {
-    settle();
-    if (threadIdx.x == 0) report_fault(p.fault);
-  }
+  if (*abort_flag) settle();
   __syncwarp();
   tcgen05_fence_before();
   cluster_meet();
+  if (threadIdx.x == 0 && *abort_flag) report_fault(p.fault);      // whichever warp's wait it was
   if (warp == 1) {
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
