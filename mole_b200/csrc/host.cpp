@@ -88,6 +88,8 @@ PyObject* guarded(F&& f) {
   try {
     return f();
   } catch (const PyRaised&) {
+  } catch (python_error& e) {            // out of Python code that torch has called, such as hooks on saved tensors
+    e.restore();
   } catch (const StatusError& e) {
     set_exception(e);
   } catch (const c10::TypeError& e) {
