@@ -473,12 +473,12 @@ int mole_adam_update(void* p, void* m, void* v, const void* g, const void* g_ext
  * all zero is a fresh state).  8-bit states are rounded up or down at random, by bits that depend on
  * (seed, t, index in the list, element) alone.  A block whose largest moment is below 2^-100 is held
  * as zeros; a moment that is NaN stays so and one that is infinite is held as its block's largest
- * code (as NaN in a block of zeros), neither touching its neighbours.  t, lr and the rest as in mole_adam_update.  The list is a
- * host array, read before the call returns.  Pointers need the alignment of their elements only; a
- * tensor whose p, g, m and v all start on 16 bytes travels by bulk copies, another one by loads of single
- * elements, several times as slow.  t and lr are taken by value, so a stream
- * under capture is refused (MOLE_ERR_STATE).  No two of the arrays that a call writes (p, m, v and the scales of all its
- * tensors) may overlap, nor a gradient what another tensor writes. */
+ * code (as NaN in a block of zeros), neither touching its neighbours.  t, lr and the rest as in
+ * mole_adam_update.  The list is a host array, read before the call returns.  Pointers need the
+ * alignment of their elements only; a tensor whose p, g, m and v all start on 16 bytes travels by bulk
+ * copies, another one by loads of single elements, three to four times as slow.  t and lr are taken by
+ * value, so a stream under capture is refused (MOLE_ERR_STATE).  No two of the arrays that a call writes
+ * (p, m, v and the scales of all its tensors) may overlap, nor a gradient what another tensor writes. */
 typedef struct {
   void* p;
   const void* g;

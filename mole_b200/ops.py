@@ -364,8 +364,9 @@ def adam_multi(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     256 consecutive elements in ``m_scales`` / ``v_scales`` (``m = code * scale``,
     ``v = (code * scale) ** 2``; zeros are a fresh state).  8-bit moments are rounded at random by
     bits that ``seed``, ``t``, the place in the list and the element determine: the same call gives
-    the same bits.  The second moment is held 4 % too large on average where gradients vary (the rounding is
-    of its root, and mean zero there).  Tensors that are written must not overlap one another."""
+    the same bits.  The second moment is held 4 % too large on average where gradients vary (the
+    rounding is of its root, and mean zero there).  Tensors that are written must not overlap one
+    another, nor the gradient of another one."""
     host.adam_multi(params, grads, exp_avgs, exp_avg_sqs, m_scales, v_scales, t, lr, betas[0], betas[1], eps,
                     weight_decay, adamw, seed)
 
